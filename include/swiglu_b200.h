@@ -65,6 +65,12 @@ extern "C" {
 #define SWIGLU_B200_ERR_LAUNCH 7      /* the kernel launch was rejected by the runtime          */
 #define SWIGLU_B200_ERR_COPY 8        /* a host<->device copy of the host-buffer entry failed  */
 #define SWIGLU_B200_ERR_WORKSPACE 9   /* the device workspace cannot hold even one token row   */
+#define SWIGLU_B200_ERR_ARG 10        /* an option (activation, group size) is none of its values */
+
+/* Activations of the entry points that take one as an argument. */
+#define SWIGLU_B200_SILU 0
+#define SWIGLU_B200_GELU_TANH 1
+#define SWIGLU_B200_GELU_ERF 2
 
 /* ABI version of this header: major*1000 + minor. */
 SWIGLU_B200_API int swiglu_b200_version(void);
@@ -293,6 +299,40 @@ SWIGLU_B200_API int swiglu_b200_lora_swiglu_fwd(void* h, void* e_out, void* g_ou
 
 /* Number of LoRA + SwiGLU epilogue kernels launched by this process. */
 SWIGLU_B200_API uint64_t swiglu_b200_lora_launch_count(void);
+
+/* Gated activation whose inputs are kept in 8 bits for the backward pass.  No counterpart in the reference,
+ * which saves gate and up as they came (kernels/swiglu/swiglu.py:326-385, kernels/geglu/geglu.py:380-575).
+ *
+ * Kept form.  Along each row, 32 consecutive columns of gate (and of up) share a step 2^(E-127): E is the biased
+ * fp32 exponent of the group's largest magnitude, plus one where that magnitude would round to 128 steps, minus 6,
+ * at least 1; an element is kept as code = rint(x / step), ties to even, in [-127, 127].  With
+ * groups = (cols + 31) / 32:
+ *   gate_codes, up_codes   int8, rows x (32 * groups), contiguous, 16-byte aligned; zero past column `cols`
+ *   gate_steps, up_steps   uint8 E, rows x groups, contiguous
+ * A group with an Inf, a NaN or a magnitude that would round to 2^128 (E above 248) has E = 255 and stands for NaN.
+ *
+ * Forward: h = act(gate*gm) * up * dm from gate and up as they came (bit-identical to swiglu_b200_fwd /
+ * swiglu_b200_geglu_fwd), and the kept form of both.  h may be NULL: the kept form alone.
+ *   h              rows x cols, row stride out_row_stride (ignored without h)
+ *   gate, up       rows x cols, row stride in_row_stride (both)
+ *   activation     SWIGLU_B200_SILU, _GELU_TANH or _GELU_ERF; the GELU forms have no multipliers (gm, dm ignored)
+ * No output may overlap an input or another output. */
+SWIGLU_B200_API int swiglu_b200_ckpt8_fwd(void* h, void* gate_codes, void* up_codes, void* gate_steps, void* up_steps,
+                          const void* gate, const void* up, int64_t rows, int64_t cols, int64_t in_row_stride,
+                          int64_t out_row_stride, int dtype, int activation, float gm, float dm, int device,
+                          void* stream);
+
+/* Backward of swiglu_b200_ckpt8_fwd from the kept form: dgate and dup as swiglu_b200_bwd / swiglu_b200_geglu_bwd
+ * give them at the values the codes stand for.
+ *   h              NULL, or rows x cols, row stride h_row_stride: act(gate*gm) * up * dm of the kept values, for a
+ *                  block that needs h again (a LoRA MLP); may overwrite dout exactly (same address, same stride)
+ *   dgate, dup     rows x cols, row stride grad_row_stride (dup = dgate + cols in the packed layout)
+ *   dout           rows x cols, row stride dout_row_stride
+ * No other overlap between an output and an input or h is allowed. */
+SWIGLU_B200_API int swiglu_b200_ckpt8_bwd(void* h, void* dgate, void* dup, const void* dout, const void* gate_codes,
+                          const void* up_codes, const void* gate_steps, const void* up_steps, int64_t rows,
+                          int64_t cols, int64_t grad_row_stride, int64_t dout_row_stride, int64_t h_row_stride,
+                          int dtype, int activation, float gm, float dm, int device, void* stream);
 
 /* Number of fused-GEMM kernels launched by this process. */
 SWIGLU_B200_API uint64_t swiglu_b200_gemm_launch_count(void);

@@ -98,6 +98,16 @@ SIGNATURES = {
         [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr,
          ctypes.c_int, _c_ptr],
     ),
+    "swiglu_b200_ckpt8_fwd": (
+        ctypes.c_int,
+        [_c_ptr] * 7 + [_c_i64] * 4 + [ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_float, ctypes.c_int,
+                                       _c_ptr],
+    ),
+    "swiglu_b200_ckpt8_bwd": (
+        ctypes.c_int,
+        [_c_ptr] * 8 + [_c_i64] * 5 + [ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_float, ctypes.c_int,
+                                       _c_ptr],
+    ),
     "swiglu_b200_gemm_bwd_launch_count": (ctypes.c_uint64, []),
     "swiglu_b200_selftest_wait_timeout": (
         ctypes.c_int, [_c_ptr, ctypes.c_int, _c_i64, ctypes.c_int, ctypes.c_int, _c_ptr]),

@@ -1,0 +1,53 @@
+// Host-side helpers shared by the C entry points: the device of a call, the library's launch counter and the
+// calling thread's last CUDA error (both kept in swiglu_capi.cu), extents of strided tensors.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace swiglu_b200 {
+
+// Counts one kernel launch in swiglu_b200_launch_count().
+void note_launch();
+// Records `e` for swiglu_b200_last_cuda_error() and returns `code`.
+int note_cuda_error(int code, cudaError_t e);
+
+// Makes `device` current for the duration of a call (no-op for -1 or when it already is).
+struct CallDevice {
+  int prev = -1;
+  bool switched = false;
+  cudaError_t err = cudaSuccess;
+  explicit CallDevice(int device) {
+    if (device < 0) return;
+    err = cudaGetDevice(&prev);
+    if (err != cudaSuccess) return;
+    if (prev != device) {
+      err = cudaSetDevice(device);
+      switched = (err == cudaSuccess);
+    }
+  }
+  ~CallDevice() {
+    if (switched) cudaSetDevice(prev);
+  }
+  CallDevice(const CallDevice&) = delete;
+  CallDevice& operator=(const CallDevice&) = delete;
+};
+
+inline unsigned long long address(const void* p) { return (unsigned long long)(uintptr_t)p; }
+
+// Bytes [lo, hi) touched by `rows` rows of `row_bytes` bytes whose starts are `pitch_bytes` apart.
+struct ByteRange {
+  unsigned long long lo, hi;
+};
+inline ByteRange byte_range(const void* p, long long rows, long long row_bytes, long long pitch_bytes) {
+  return ByteRange{address(p), address(p) + (unsigned long long)((rows - 1) * pitch_bytes + row_bytes)};
+}
+inline bool overlap(const ByteRange& a, const ByteRange& b) { return a.lo < b.hi && b.lo < a.hi; }
+
+// True when rows * pitch (in bytes) and everything derived from it stays within 62 bits.
+inline bool fits_address_space(long long rows, long long pitch, long long element) {
+  if (pitch > (1LL << 56) || rows > (1LL << 56)) return false;
+  return rows == 0 || pitch * element <= (1LL << 62) / rows;
+}
+
+}  // namespace swiglu_b200

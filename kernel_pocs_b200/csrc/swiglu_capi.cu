@@ -4,6 +4,7 @@
 
 #include <atomic>
 
+#include "launch_common.cuh"
 #include "swiglu_kernels.cuh"
 
 namespace {
@@ -402,6 +403,11 @@ inline bool overlaps(const Extent& a, const Extent& b) { return a.lo < b.hi && b
 
 }  // namespace
 
+namespace swiglu_b200 {
+void note_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
+int note_cuda_error(int code, cudaError_t e) { return fail_cuda(code, e); }
+}  // namespace swiglu_b200
+
 extern "C" {
 
 int swiglu_b200_version(void) { return 1000; }
@@ -418,6 +424,7 @@ const char* swiglu_b200_strerror(int code) {
     case SWIGLU_B200_ERR_LAUNCH: return "CUDA kernel launch failed";
     case SWIGLU_B200_ERR_COPY: return "CUDA host<->device copy failed";
     case SWIGLU_B200_ERR_WORKSPACE: return "device workspace too small for one chunk of token rows";
+    case SWIGLU_B200_ERR_ARG: return "an option (activation, group size) is none of its values";
     default: return "unknown swiglu_b200 error code";
   }
 }
