@@ -1,0 +1,281 @@
+"""Gated MLP with 4-bit weights for a few tokens: the frozen projections of a block that generates.
+
+With one token, or one per sequence of a small batch, an MLP costs what it takes to read its weights.  Here they are
+4-bit codes with a scale (and, optionally, a zero point) for every ``group_size`` columns, and are turned back into
+numbers inside the kernel that multiplies them:
+
+    w4_linear(x, w)                      x W^T
+    w4_gate_up(x, w_gate, w_up, ...)     act(x Wg^T * gm) * (x Wu^T) * dm in one launch
+    w4_mlp(x, w_gate, w_up, w_down, ...) both, one after the other
+    quantize_w4(weight, ...)             a ``W4Weight`` from a bf16 / fp16 matrix
+    W4Weight(packed, scales, zeros, ...) one from codes that exist already
+
+W[n, k] is ``(code - zero) * scale``; products with x are summed in fp32 and scaled in fp32, and the result is rounded
+once to the dtype of x.  ``MATVEC_ROWS`` tokens and fewer take these kernels; more (a prompt) take the weights written
+out in 16 bits by ``W4Weight.dequantize`` and the tensor-core projections of ``fused_mlp`` / ``geglu``, whose
+operands then carry one more rounding (half a unit of the 16-bit type per weight).  Forward only: weights are frozen and
+an input that wants a gradient is refused.  The reference has no counterpart (its inference path is bf16,
+kernels/lora_mlp/experiments/v5/lora_mlp_kernel_v5.py:451-454).  There is no path for tensors that are not on a CUDA
+device.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .checkpoint8 import ACTIVATIONS, _check_activation, _check_multipliers, _pitch, _rows
+from .swiglu import _DTYPE_CODE, _stream
+
+DTYPES = (torch.bfloat16, torch.float16)
+GROUP_SIZES = (32, 64, 128)
+TILE_ROWS, TILE_COLS = 16, 128
+MATVEC_ROWS = 32
+
+
+def _ceil(a: int, b: int) -> int:
+    return (a + b - 1) // b
+
+
+class W4Weight:
+    """A ``[out_features, in_features]`` matrix in 4 bits.
+
+    ``packed``  uint8 ``[n, 16 * ceil(k / 32)]``: byte j of a row holds the codes of columns 2j (low half) and 2j + 1;
+    ``scales``  bf16 or fp16 ``[n, ceil(k / group_size)]``, the dtype of the tokens it multiplies;
+    ``zeros``   uint8 of the shape of ``scales``, 0..15, or ``None`` for 8 everywhere.
+
+    The constructor lays them out once in the tiles the kernels read (``swiglu_b200_w4_linear`` in the C header) and
+    keeps only those; ``packed``, ``scales`` and ``zeros`` are rebuilt on request."""
+
+    __slots__ = ("tiles", "tile_scales", "tile_zeros", "out_features", "in_features", "group_size")
+
+    def __init__(self, packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, *,
+                 in_features: int, group_size: int = 128):
+        if group_size not in GROUP_SIZES:
+            raise ValueError(f"group_size must be one of {GROUP_SIZES}, got {group_size}")
+        if packed.dim() != 2 or packed.shape[0] < 1 or in_features < 1:
+            raise ValueError("packed must be a [n, bytes] matrix of at least one row and one column")
+        n, k = packed.shape[0], int(in_features)
+        if packed.dtype != torch.uint8:
+            raise TypeError(f"packed must be uint8, got {packed.dtype}")
+        if packed.shape[1] != 16 * _ceil(k, 32):
+            raise ValueError(f"packed needs {16 * _ceil(k, 32)} bytes per row for {k} columns, got {packed.shape[1]}")
+        if scales.dtype not in DTYPES:
+            raise TypeError(f"scales must be bf16 or fp16, got {scales.dtype}")
+        if scales.shape != (n, _ceil(k, group_size)):
+            raise ValueError(f"scales must be of shape {(n, _ceil(k, group_size))}, got {tuple(scales.shape)}")
+        if zeros is not None:
+            if zeros.dtype != torch.uint8:
+                raise TypeError(f"zeros must be uint8, got {zeros.dtype}")
+            if zeros.shape != scales.shape:
+                raise ValueError(f"zeros must be of shape {tuple(scales.shape)}, got {tuple(zeros.shape)}")
+            if int(zeros.max()) > 15:
+                raise ValueError("zeros must lie in 0..15")
+        if any(t is not None and t.device != packed.device for t in (scales, zeros)):
+            raise ValueError("packed, scales and zeros must be on one device")
+        self.out_features, self.in_features, self.group_size = n, k, group_size
+        rows, cols = _ceil(n, TILE_ROWS), _ceil(k, TILE_COLS)
+        # [row tile, 2, 8, column tile, word u, lane t, byte] -> [row tile, column tile, 2, 8, t, u, byte]
+        p = torch.nn.functional.pad(packed, (0, 64 * cols - packed.shape[1], 0, TILE_ROWS * rows - n))
+        self.tiles = p.reshape(rows, 2, 8, cols, 4, 4, 4).permute(0, 3, 1, 2, 5, 4, 6).contiguous()
+        self.tile_scales = self._tile_groups(scales)
+        self.tile_zeros = None if zeros is None else self._tile_groups(zeros)
+
+    def _groups(self) -> int:
+        return _ceil(self.in_features, TILE_COLS) * (TILE_COLS // self.group_size)
+
+    def _tile_groups(self, t: torch.Tensor) -> torch.Tensor:
+        """[n, groups] -> [row tile, group, 8, 2], zero past the matrix."""
+        rows, groups = self.tiles.shape[0], self._groups()
+        t = torch.nn.functional.pad(t, (0, groups - t.shape[1], 0, TILE_ROWS * rows - t.shape[0]))
+        return t.reshape(rows, 2, 8, groups).permute(0, 3, 2, 1).contiguous()
+
+    def _untile_groups(self, t: torch.Tensor) -> torch.Tensor:
+        rows = t.permute(0, 3, 2, 1).reshape(-1, self._groups())
+        return rows[:self.out_features, :_ceil(self.in_features, self.group_size)].contiguous()
+
+    @property
+    def packed(self) -> torch.Tensor:
+        rows, cols = self.tiles.shape[:2]
+        p = self.tiles.permute(0, 2, 3, 1, 5, 4, 6).reshape(TILE_ROWS * rows, 64 * cols)
+        return p[:self.out_features, :16 * _ceil(self.in_features, 32)].contiguous()
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._untile_groups(self.tile_scales)
+
+    @property
+    def zeros(self) -> Optional[torch.Tensor]:
+        return None if self.tile_zeros is None else self._untile_groups(self.tile_zeros)
+
+    @property
+    def shape(self) -> torch.Size:
+        return torch.Size((self.out_features, self.in_features))
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return self.tile_scales.dtype
+
+    @property
+    def device(self) -> torch.device:
+        return self.tiles.device
+
+    @property
+    def nbytes(self) -> int:
+        """Bytes the kernels read of it."""
+        parts = (self.tiles, self.tile_scales, self.tile_zeros)
+        return sum(t.numel() * t.element_size() for t in parts if t is not None)
+
+    def to(self, device) -> "W4Weight":
+        """This weight on ``device`` (itself when it is there already)."""
+        moved = self.tiles.to(device)
+        if moved is self.tiles:
+            return self
+        other = object.__new__(W4Weight)
+        other.out_features, other.in_features, other.group_size = self.out_features, self.in_features, self.group_size
+        other.tiles, other.tile_scales = moved, self.tile_scales.to(device)
+        other.tile_zeros = None if self.tile_zeros is None else self.tile_zeros.to(device)
+        return other
+
+    def _pointers(self):
+        return (self.tiles.data_ptr(), self.tile_scales.data_ptr(),
+                None if self.tile_zeros is None else self.tile_zeros.data_ptr())
+
+    def dequantize(self) -> torch.Tensor:
+        """``[out_features, in_features]`` in the dtype of the scales: ``(code - zero) * scale`` rounded once."""
+        if not self.tiles.is_cuda:
+            raise RuntimeError("W4Weight.dequantize has a CUDA (sm_100a) kernel only; there is no CPU fallback")
+        n, k = self.shape
+        out = torch.empty((n, k), dtype=self.dtype, device=self.device)
+        _lib.check(
+            "W4Weight.dequantize",
+            _lib.lib.swiglu_b200_w4_dequantize(out.data_ptr(), *self._pointers(), n, k, k, self.group_size,
+                                               _DTYPE_CODE[self.dtype], self.device.index, _stream(self.device)),
+        )
+        return out
+
+
+def quantize_w4(weight: torch.Tensor, group_size: int = 128, zero_points: bool = False,
+                dtype: Optional[torch.dtype] = None) -> W4Weight:
+    """``weight`` ``[n, k]`` in 4 bits, rounded to nearest.  Every ``group_size`` columns of a row share a scale of
+    ``dtype`` (the weight's own by default): the group's largest magnitude over 7, or with ``zero_points`` its range
+    (zero included) over 15."""
+    if group_size not in GROUP_SIZES:
+        raise ValueError(f"group_size must be one of {GROUP_SIZES}, got {group_size}")
+    if weight.dim() != 2 or weight.numel() == 0:
+        raise ValueError(f"weight must be a non-empty matrix, got shape {tuple(weight.shape)}")
+    dtype = weight.dtype if dtype is None else dtype
+    if dtype not in DTYPES or not weight.is_floating_point():
+        raise TypeError(f"4-bit weights carry bf16 or fp16 scales, got {dtype}")
+    n, k = weight.shape
+    if not bool(torch.isfinite(weight).all()):
+        raise ValueError("weight holds values that are not finite")
+    groups, pitch = _ceil(k, group_size), 32 * _ceil(k, 32)
+    packed = torch.empty((n, pitch // 2), dtype=torch.uint8, device=weight.device)
+    scales = torch.empty((n, groups), dtype=dtype, device=weight.device)
+    zeros = torch.empty((n, groups), dtype=torch.uint8, device=weight.device) if zero_points else None
+    step = max(1, (1 << 26) // (groups * group_size))  # rows at a time: a quarter of a gigabyte of fp32
+    for lo in range(0, n, step):
+        w = weight[lo:lo + step].detach().to(torch.float32)
+        rows = w.shape[0]
+        w = torch.nn.functional.pad(w, (0, groups * group_size - k)).view(rows, groups, group_size)
+        if zero_points:
+            low, high = w.amin(-1).clamp(max=0), w.amax(-1).clamp(min=0)
+            scale = ((high - low) / 15).to(dtype)
+        else:
+            scale = (w.abs().amax(-1) / 7).to(dtype)
+        if not bool(torch.isfinite(scale).all()):
+            raise ValueError(f"weight holds magnitudes whose scale is not a finite {dtype}")
+        inverse = torch.where(scale > 0, 1.0 / scale.to(torch.float32), 0.0)
+        if zero_points:
+            zero = torch.round(-low * inverse).clamp(0, 15)
+            zeros[lo:lo + step] = zero.to(torch.uint8)
+        else:
+            zero = torch.full_like(inverse, 8.0)
+        code = (torch.round(w * inverse.unsqueeze(-1)) + zero.unsqueeze(-1)).clamp(0, 15).to(torch.uint8)
+        code = torch.nn.functional.pad(code.view(rows, -1), (0, max(0, pitch - groups * group_size)))[:, :pitch]
+        packed[lo:lo + step] = code[:, 0::2] | (code[:, 1::2] << 4)
+        scales[lo:lo + step] = scale
+    return W4Weight(packed, scales, zeros, in_features=k, group_size=group_size)
+
+
+def _check_tokens(x: torch.Tensor, w: W4Weight, what: str) -> None:
+    if not (x.is_cuda and w.tiles.is_cuda):
+        raise RuntimeError(f"{what} has a CUDA (sm_100a) kernel only; there is no CPU fallback")
+    if x.device != w.device:
+        raise ValueError(f"x is on {x.device}, the weight on {w.device}")
+    if x.dtype != w.dtype:
+        raise TypeError(f"x is {x.dtype}, the weight's scales are {w.dtype}")
+    if x.dim() == 0 or x.shape[-1] != w.in_features:
+        raise ValueError(f"x of shape {tuple(x.shape)} does not end in the weight's {w.in_features} features")
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise RuntimeError(f"{what} is forward only (frozen 4-bit weights): call it under torch.no_grad()")
+
+
+def w4_linear(x: torch.Tensor, weight: W4Weight) -> torch.Tensor:
+    """``x W^T`` for ``x`` ``[..., in_features]`` of the weight's dtype."""
+    _check_tokens(x, weight, "w4_linear")
+    n, k = weight.shape
+    x2 = _rows(x)
+    m = x2.shape[0]
+    if m > MATVEC_ROWS:
+        return (x2 @ weight.dequantize().t()).view(*x.shape[:-1], n)
+    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    _lib.check(
+        "w4_linear",
+        _lib.lib.swiglu_b200_w4_linear(y.data_ptr(), x2.data_ptr(), *weight._pointers(), m, n, k, _pitch(x2), n,
+                                       weight.group_size, _DTYPE_CODE[x.dtype], x.device.index, _stream(x.device)),
+    )
+    return y.view(*x.shape[:-1], n)
+
+
+def _gate_up_16bit(x, w_gate, w_up, activation, gm, dm):
+    """The same stage from weights written out in 16 bits, for more tokens than the 4-bit kernel is for."""
+    from .fused_mlp import gate_up_swiglu_forward
+    from .geglu import gate_up_geglu_forward, geglu_forward
+    from .swiglu import swiglu_forward
+
+    wg, wu = w_gate.dequantize(), w_up.dequantize()
+    n, k = wg.shape
+    approximate = "tanh" if activation == "gelu_tanh" else "none"
+    if x.dtype == torch.bfloat16 and k % 8 == 0 and n % 16 == 0:
+        if activation == "silu":
+            return gate_up_swiglu_forward(x, wg, wu, gm, dm)
+        return gate_up_geglu_forward(x, wg, wu, approximate)
+    gate, up = x @ wg.t(), x @ wu.t()
+    return swiglu_forward(gate, up, gm, dm)[0] if activation == "silu" else geglu_forward(gate, up, approximate)[0]
+
+
+def w4_gate_up(x: torch.Tensor, w_gate: W4Weight, w_up: W4Weight, activation: str = "silu",
+               gate_multiplier: float = 1.0, down_multiplier: float = 1.0) -> torch.Tensor:
+    """``act(x Wg^T * gate_multiplier) * (x Wu^T) * down_multiplier``; both projections and the activation (``"silu"``,
+    ``"gelu_tanh"`` or ``"gelu_exact"``; the GELU forms have no multipliers) in one launch, neither projection rounded
+    on the way."""
+    _check_activation(activation)
+    gm, dm = _check_multipliers(activation, gate_multiplier, down_multiplier)
+    if w_gate.shape != w_up.shape or w_gate.group_size != w_up.group_size or w_gate.dtype != w_up.dtype:
+        raise ValueError("w_gate and w_up must agree in shape, group size and dtype")
+    _check_tokens(x, w_gate, "w4_gate_up")
+    _check_tokens(x, w_up, "w4_gate_up")
+    n, k = w_gate.shape
+    x2 = _rows(x)
+    m = x2.shape[0]
+    if m > MATVEC_ROWS:
+        return _gate_up_16bit(x, w_gate, w_up, activation, gm, dm)
+    h = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    _lib.check(
+        "w4_gate_up",
+        _lib.lib.swiglu_b200_w4_gate_up(
+            h.data_ptr(), x2.data_ptr(), *w_gate._pointers(), *w_up._pointers(), m, n, k, _pitch(x2), n,
+            w_gate.group_size, _DTYPE_CODE[x.dtype], ACTIVATIONS[activation], gm, dm, x.device.index,
+            _stream(x.device),
+        ),
+    )
+    return h.view(*x.shape[:-1], n)
+
+
+def w4_mlp(x: torch.Tensor, w_gate: W4Weight, w_up: W4Weight, w_down: W4Weight,
+           activation: str = "silu") -> torch.Tensor:
+    """``down(act(gate(x)) * up(x))`` with all three projections in 4 bits: two launches for a few tokens."""
+    return w4_linear(w4_gate_up(x, w_gate, w_up, activation), w_down)
