@@ -150,9 +150,8 @@ def _load() -> ctypes.CDLL:
 
 
 class _LazyLibrary:
-    """Stands for the bound library; binds it the first time an entry point is looked up."""
-
-    __slots__ = ("_cdll",)
+    """Stands for the bound library; binds it the first time an entry point is looked up.  Entry points become
+    attributes on first use, so that later look-ups cost no call."""
 
     def __init__(self):
         self._cdll = None
@@ -163,7 +162,9 @@ class _LazyLibrary:
         return self._cdll
 
     def __getattr__(self, name: str):
-        return getattr(self._bound(), name)
+        fn = getattr(self._bound(), name)
+        setattr(self, name, fn)
+        return fn
 
 
 lib = _LazyLibrary()

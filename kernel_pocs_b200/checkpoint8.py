@@ -41,35 +41,69 @@ GROUP = 32
 class Checkpoint8:
     """gate and up of one forward pass in 8 bits.
 
-    ``codes`` int8 ``[2, rows, 32 * groups]`` and ``steps`` uint8 ``[2, rows, groups]`` (gate first), with the shape and
-    dtype of the inputs and what the backward needs of the call: the activation and its multipliers."""
+    ``data`` is one uint8 buffer of ``Checkpoint8.size(shape)`` bytes: the codes of gate, the codes of up, the steps of
+    gate, the steps of up.  With it go the shape and dtype of the inputs and what the backward needs of the call: the
+    activation and its multipliers.  ``codes`` (int8 ``[2, rows, 32 * groups]``) and ``steps`` (uint8
+    ``[2, rows, groups]``), gate first, are views of ``data``."""
 
-    __slots__ = ("codes", "steps", "shape", "dtype", "activation", "gate_multiplier", "down_multiplier")
+    __slots__ = ("data", "shape", "dtype", "activation", "gate_multiplier", "down_multiplier")
 
-    def __init__(self, codes, steps, shape, dtype, activation="silu", gate_multiplier=1.0, down_multiplier=1.0):
-        self.codes = codes
-        self.steps = steps
-        self.shape = torch.Size(shape)
+    def __init__(self, data, shape, dtype, activation="silu", gate_multiplier=1.0, down_multiplier=1.0):
+        shape = torch.Size(shape)
+        if data.dtype != torch.uint8 or data.dim() != 1 or data.numel() != Checkpoint8.size(shape):
+            raise ValueError(f"the kept form of shape {tuple(shape)} is {Checkpoint8.size(shape)} bytes")
+        self.data = data
+        self.shape = shape
         self.dtype = dtype
         self.activation = _check_activation(activation)
         self.gate_multiplier, self.down_multiplier = _check_multipliers(activation, gate_multiplier, down_multiplier)
 
+    @staticmethod
+    def _of(data, shape, dtype, activation, gm, dm) -> "Checkpoint8":
+        """One whose parts have been checked."""
+        kept = object.__new__(Checkpoint8)
+        kept.data, kept.shape, kept.dtype = data, shape, dtype
+        kept.activation, kept.gate_multiplier, kept.down_multiplier = activation, gm, dm
+        return kept
+
+    @staticmethod
+    def size(shape) -> int:
+        """Bytes of the kept form of gate and up of this shape."""
+        rows, _, groups = _sizes(torch.Size(shape))
+        return 2 * rows * groups * (GROUP + 1)
+
+    @property
+    def codes(self) -> torch.Tensor:
+        rows, _, groups = _sizes(self.shape)
+        return self.data[:2 * rows * groups * GROUP].view(torch.int8).view(2, rows, groups * GROUP)
+
+    @property
+    def steps(self) -> torch.Tensor:
+        rows, _, groups = _sizes(self.shape)
+        return self.data[2 * rows * groups * GROUP:].view(2, rows, groups)
+
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self.data.device
 
     @property
     def nbytes(self) -> int:
-        return self.codes.numel() + self.steps.numel()
+        return self.data.numel()
 
     def dequantize(self) -> Tuple[torch.Tensor, torch.Tensor]:
         """The values that the codes of gate and up stand for, in fp32 and the inputs' shape."""
+        rows, n_cols, groups = _sizes(self.shape)
         exponent = self.steps.to(torch.int32)
         step = torch.where(exponent == 255, 0x7fc00000, exponent << 23).view(torch.float32)
-        values = self.codes.view(*self.steps.shape, GROUP).to(torch.float32) * step.unsqueeze(-1)
-        n_cols = self.shape[-1]
-        values = values.view(self.codes.shape)[:, :, :n_cols].reshape(2, *self.shape)
+        values = self.codes.view(2, rows, groups, GROUP).to(torch.float32) * step.unsqueeze(-1)
+        values = values.view(2, rows, groups * GROUP)[:, :, :n_cols].reshape(2, *self.shape)
         return values[0], values[1]
+
+
+def _sizes(shape: torch.Size) -> Tuple[int, int, int]:
+    """Rows, columns and groups per row of inputs of this shape."""
+    n_cols = shape[-1]
+    return shape.numel() // n_cols if n_cols else 0, n_cols, (n_cols + GROUP - 1) // GROUP
 
 
 def _check_activation(activation: str) -> str:
@@ -107,40 +141,47 @@ def _row_view(x: torch.Tensor) -> Optional[torch.Tensor]:
     return v
 
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
+def _rows(x: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """A tensor whose storage holds the rows of ``x`` in order (``x`` itself, or a copy), and their pitch."""
+    if x.is_contiguous():
+        return x, x.shape[-1]
     v = _row_view(x)
-    return _row_view(x.contiguous()) if v is None else v
+    return (x.contiguous(), x.shape[-1]) if v is None else (v, _pitch(v))
 
 
 def _pitch(v: torch.Tensor) -> int:
     return v.stride(0) if v.shape[0] > 1 else v.shape[1]
 
 
-def _input_rows(gate: torch.Tensor, up: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+def _input_rows(gate: torch.Tensor, up: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, int]:
     """Both as rows of one pitch: in place when they are (two halves of a packed projection), else copied."""
-    g, u = _row_view(gate), _row_view(up)
-    if g is not None and u is not None and _pitch(g) == _pitch(u):
-        return g, u
-    return _row_view(gate.contiguous()), _row_view(up.contiguous())
+    if not (gate.is_contiguous() and up.is_contiguous()):
+        g, u = _row_view(gate), _row_view(up)
+        if g is not None and u is not None and _pitch(g) == _pitch(u):
+            return g, u, _pitch(g)
+        gate, up = gate.contiguous(), up.contiguous()
+    return gate, up, gate.shape[-1]
 
 
-def _keep(gate_2d, up_2d, shape, activation, gm, dm, want_h: bool, where: str):
-    rows, n_cols = gate_2d.shape
-    groups = (n_cols + GROUP - 1) // GROUP
-    device, dtype = gate_2d.device, gate_2d.dtype
-    codes = torch.empty((2, rows, groups * GROUP), dtype=torch.int8, device=device)
-    steps = torch.empty((2, rows, groups), dtype=torch.uint8, device=device)
-    h = torch.empty((rows, n_cols), dtype=dtype, device=device) if want_h else None
+def _keep(gate, up, activation, gm, dm, want_h: bool, where: str):
+    _check_inputs(gate, up)
+    shape, dtype, device = gate.shape, gate.dtype, gate.device
+    rows, n_cols, groups = _sizes(shape)
+    gate, up, pitch = _input_rows(gate, up)
     plane, plane_steps = rows * groups * GROUP, rows * groups
+    data = torch.empty(2 * (plane + plane_steps), dtype=torch.uint8, device=device)
+    h = torch.empty(shape, dtype=dtype, device=device) if want_h else None
+    base = data.data_ptr()
+    steps = base + 2 * plane
     _lib.check(
         where,
         _lib.lib.swiglu_b200_ckpt8_fwd(
-            h.data_ptr() if want_h else None, codes.data_ptr(), codes.data_ptr() + plane, steps.data_ptr(),
-            steps.data_ptr() + plane_steps, gate_2d.data_ptr(), up_2d.data_ptr(), rows, n_cols, _pitch(gate_2d),
-            n_cols, _DTYPE_CODE[dtype], ACTIVATIONS[activation], gm, dm, device.index, _stream(device),
+            h.data_ptr() if want_h else None, base, base + plane, steps, steps + plane_steps, gate.data_ptr(),
+            up.data_ptr(), rows, n_cols, pitch, n_cols, _DTYPE_CODE[dtype], ACTIVATIONS[activation], gm, dm,
+            device.index, _stream(device),
         ),
     )
-    return h, Checkpoint8(codes, steps, shape, dtype, activation, gm, dm)
+    return h, Checkpoint8._of(data, shape, dtype, activation, gm, dm)
 
 
 def ckpt8_forward(gate: torch.Tensor, up: torch.Tensor, activation: str = "silu", gate_multiplier: float = 1.0,
@@ -150,10 +191,7 @@ def ckpt8_forward(gate: torch.Tensor, up: torch.Tensor, activation: str = "silu"
     place."""
     _check_activation(activation)
     gm, dm = _check_multipliers(activation, gate_multiplier, down_multiplier)
-    _check_inputs(gate, up)
-    gate_2d, up_2d = _input_rows(gate, up)
-    h, kept = _keep(gate_2d, up_2d, gate.shape, activation, gm, dm, True, "ckpt8_forward")
-    return h.view(gate.shape), kept
+    return _keep(gate, up, activation, gm, dm, True, "ckpt8_forward")
 
 
 def ckpt8_pack(gate: torch.Tensor, up: torch.Tensor, activation: str = "silu", gate_multiplier: float = 1.0,
@@ -161,9 +199,24 @@ def ckpt8_pack(gate: torch.Tensor, up: torch.Tensor, activation: str = "silu", g
     """The ``Checkpoint8`` alone, for a block whose own kernel has made ``h`` (the fused projections)."""
     _check_activation(activation)
     gm, dm = _check_multipliers(activation, gate_multiplier, down_multiplier)
-    _check_inputs(gate, up)
-    gate_2d, up_2d = _input_rows(gate, up)
-    return _keep(gate_2d, up_2d, gate.shape, activation, gm, dm, False, "ckpt8_pack")[1]
+    return _keep(gate, up, activation, gm, dm, False, "ckpt8_pack")[1]
+
+
+def _gradients(dout, kept: Checkpoint8, dgate: int, dup: int, grad_pitch: int, h, where: str) -> None:
+    """Fills dgate and dup (addresses of rows ``grad_pitch`` apart), and ``h`` when it is given."""
+    rows, n_cols, groups = _sizes(kept.shape)
+    dout, pitch = _rows(dout)
+    codes, plane, plane_steps = kept.data.data_ptr(), rows * groups * GROUP, rows * groups
+    steps = codes + 2 * plane
+    device = kept.device
+    _lib.check(
+        where,
+        _lib.lib.swiglu_b200_ckpt8_bwd(
+            h.data_ptr() if h is not None else None, dgate, dup, dout.data_ptr(), codes, codes + plane, steps,
+            steps + plane_steps, rows, n_cols, grad_pitch, pitch, n_cols, _DTYPE_CODE[kept.dtype],
+            ACTIVATIONS[kept.activation], kept.gate_multiplier, kept.down_multiplier, device.index, _stream(device),
+        ),
+    )
 
 
 def _check_dout(dout: torch.Tensor, kept: Checkpoint8) -> None:
@@ -171,32 +224,14 @@ def _check_dout(dout: torch.Tensor, kept: Checkpoint8) -> None:
         raise TypeError("dout must have the dtype and device of gate and up")
     if dout.shape != kept.shape:
         raise ValueError(f"dout of shape {tuple(dout.shape)} does not match gate of shape {tuple(kept.shape)}")
-
-
-def _gradients(dout_2d, kept: Checkpoint8, dgate, dup, grad_pitch: int, h, where: str) -> None:
-    """Fills dgate and dup (addresses of rows ``grad_pitch`` apart), and ``h`` when it is given."""
-    _, rows, groups = kept.steps.shape
-    n_cols = kept.shape[-1]
-    codes, steps = kept.codes.data_ptr(), kept.steps.data_ptr()
-    device = kept.device
-    _lib.check(
-        where,
-        _lib.lib.swiglu_b200_ckpt8_bwd(
-            h.data_ptr() if h is not None else None, dgate, dup, dout_2d.data_ptr(), codes,
-            codes + rows * groups * GROUP, steps, steps + rows * groups, rows, n_cols, grad_pitch, _pitch(dout_2d),
-            _pitch(h) if h is not None else 0, _DTYPE_CODE[kept.dtype], ACTIVATIONS[kept.activation],
-            kept.gate_multiplier, kept.down_multiplier, device.index, _stream(device),
-        ),
-    )
+    _require_cuda(dout, "dout")
 
 
 def ckpt8_backward(dout: torch.Tensor, kept: Checkpoint8):
     """``(dgate, dup)`` of a ``ckpt8_forward`` / ``ckpt8_pack``, in the inputs' shape."""
     _check_dout(dout, kept)
-    dout_2d = _rows(dout)
-    n_cols = kept.shape[-1]
-    dgate, dup = (torch.empty(kept.shape, dtype=kept.dtype, device=kept.device) for _ in range(2))
-    _gradients(dout_2d, kept, dgate.data_ptr(), dup.data_ptr(), n_cols, None, "ckpt8_backward")
+    dgate, dup = dout.new_empty(kept.shape), dout.new_empty(kept.shape)
+    _gradients(dout, kept, dgate.data_ptr(), dup.data_ptr(), kept.shape[-1], None, "ckpt8_backward")
     return dgate, dup
 
 
@@ -204,33 +239,29 @@ def ckpt8_backward_recompute(dout: torch.Tensor, kept: Checkpoint8, preserve_inp
     """``(h, dgate, dup)`` in one pass: the gradients together with ``act(gate * gm) * up * dm`` of the kept values, as
     ``swiglu_backward_recompute`` gives them from gate and up.  Unless ``preserve_inputs`` is set, ``h`` is written
     over ``dout``, which must be contiguous then."""
+    if not (preserve_inputs or dout.is_contiguous()):
+        raise ValueError("the in-place form needs a contiguous dout; pass preserve_inputs=True")
     _check_dout(dout, kept)
-    if preserve_inputs:
-        dout_2d = _rows(dout)
-        h = torch.empty(dout_2d.shape, dtype=kept.dtype, device=kept.device)
-    else:
-        if not dout.is_contiguous():
-            raise ValueError("the in-place form needs a contiguous dout; pass preserve_inputs=True")
-        dout_2d = h = _rows(dout)
-    dgate, dup = (torch.empty(kept.shape, dtype=kept.dtype, device=kept.device) for _ in range(2))
-    _gradients(dout_2d, kept, dgate.data_ptr(), dup.data_ptr(), kept.shape[-1], h, "ckpt8_backward_recompute")
-    return (h.view(kept.shape) if preserve_inputs else dout), dgate, dup
+    h = dout.new_empty(kept.shape) if preserve_inputs else dout
+    dgate, dup = dout.new_empty(kept.shape), dout.new_empty(kept.shape)
+    _gradients(dout, kept, dgate.data_ptr(), dup.data_ptr(), kept.shape[-1], h, "ckpt8_backward_recompute")
+    return h, dgate, dup
 
 
 class ForgeCkpt8Function(torch.autograd.Function):
-    """``apply(gate, up, activation="silu", gate_multiplier=1.0, down_multiplier=1.0)``; saves the codes and steps."""
+    """``apply(gate, up, activation="silu", gate_multiplier=1.0, down_multiplier=1.0)``; saves the kept form."""
 
     @staticmethod
     def forward(ctx, gate, up, activation="silu", gate_multiplier=1.0, down_multiplier=1.0):
         h, kept = ckpt8_forward(gate, up, activation, gate_multiplier, down_multiplier)
-        ctx.save_for_backward(kept.codes, kept.steps)
+        ctx.save_for_backward(kept.data)
         ctx.call = (kept.shape, kept.dtype, kept.activation, kept.gate_multiplier, kept.down_multiplier)
         return h
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        dgate, dup = ckpt8_backward(dout, Checkpoint8(*ctx.saved_tensors, *ctx.call))
+        dgate, dup = ckpt8_backward(dout, Checkpoint8._of(*ctx.saved_tensors, *ctx.call))
         return dgate, dup, None, None, None
 
 
@@ -244,19 +275,19 @@ class ForgePackedCkpt8Function(torch.autograd.Function):
         packed = gate_up if _row_view(gate_up) is not None else gate_up.contiguous()
         h, kept = ckpt8_forward(packed[..., :n_cols], packed[..., n_cols:], activation, gate_multiplier,
                                 down_multiplier)
-        ctx.save_for_backward(kept.codes, kept.steps)
+        ctx.save_for_backward(kept.data)
         ctx.call = (kept.shape, kept.dtype, kept.activation, kept.gate_multiplier, kept.down_multiplier)
         return h
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        kept = Checkpoint8(*ctx.saved_tensors, *ctx.call)
+        kept = Checkpoint8._of(*ctx.saved_tensors, *ctx.call)
         _check_dout(dout, kept)
         n_cols = kept.shape[-1]
-        grad = torch.empty((*kept.shape[:-1], 2 * n_cols), dtype=kept.dtype, device=kept.device)
+        grad = dout.new_empty((*kept.shape[:-1], 2 * n_cols))
         base = grad.data_ptr()
-        _gradients(_rows(dout), kept, base, base + n_cols * grad.element_size(), 2 * n_cols, None,
+        _gradients(dout, kept, base, base + n_cols * grad.element_size(), 2 * n_cols, None,
                    "packed ckpt8_backward")
         return grad, None, None, None
 
@@ -268,11 +299,9 @@ def _records(*inputs: torch.Tensor) -> bool:
 def swiglu_ckpt8(gate: torch.Tensor, up: torch.Tensor, gate_multiplier: float = 1.0,
                  down_multiplier: float = 1.0) -> torch.Tensor:
     """``swiglu`` that keeps gate and up in 8 bits for its backward (nothing is kept when no gradient is wanted)."""
-    _check_same_shape_inputs(gate, up)
-    _check_multipliers("silu", gate_multiplier, down_multiplier)
-    _require_cuda(gate, "gate")
     if not _records(gate, up):
-        return swiglu_forward(gate, up, gate_multiplier, down_multiplier)[0]
+        gm, dm = _check_multipliers("silu", gate_multiplier, down_multiplier)
+        return swiglu_forward(gate, up, gm, dm)[0]
     return ForgeCkpt8Function.apply(gate, up, "silu", gate_multiplier, down_multiplier)
 
 
@@ -280,10 +309,9 @@ def swiglu_packed_ckpt8(gate_up: torch.Tensor, gate_multiplier: float = 1.0,
                         down_multiplier: float = 1.0) -> torch.Tensor:
     """``swiglu_packed`` that keeps both halves in 8 bits for its backward."""
     _check_packed_input(gate_up)
-    _check_multipliers("silu", gate_multiplier, down_multiplier)
-    _require_cuda(gate_up, "gate_up")
     if not _records(gate_up):
-        return swiglu_packed_forward(gate_up, gate_multiplier, down_multiplier)[0]
+        gm, dm = _check_multipliers("silu", gate_multiplier, down_multiplier)
+        return swiglu_packed_forward(gate_up, gm, dm)[0]
     return ForgePackedCkpt8Function.apply(gate_up, "silu", gate_multiplier, down_multiplier)
 
 
@@ -293,9 +321,7 @@ def _gelu(approximate: str) -> str:
 
 def geglu_ckpt8(gate: torch.Tensor, up: torch.Tensor, approximate: str = "tanh") -> torch.Tensor:
     """``geglu`` that keeps gate and up in 8 bits for its backward (nothing is kept when no gradient is wanted)."""
-    _check_same_shape_inputs(gate, up)
     activation = _gelu(approximate)
-    _require_cuda(gate, "gate")
     if not _records(gate, up):
         return geglu_forward(gate, up, approximate)[0]
     return ForgeCkpt8Function.apply(gate, up, activation)
@@ -305,7 +331,6 @@ def geglu_packed_ckpt8(gate_up: torch.Tensor, approximate: str = "tanh") -> torc
     """``geglu_packed`` that keeps both halves in 8 bits for its backward."""
     _check_packed_input(gate_up)
     activation = _gelu(approximate)
-    _require_cuda(gate_up, "gate_up")
     if not _records(gate_up):
         return geglu_packed_forward(gate_up, approximate)[0]
     return ForgePackedCkpt8Function.apply(gate_up, activation)

@@ -25,7 +25,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .checkpoint8 import ACTIVATIONS, _check_activation, _check_multipliers, _pitch, _rows
+from .checkpoint8 import ACTIVATIONS, _check_activation, _check_multipliers, _rows
 from .swiglu import _DTYPE_CODE, _stream
 
 DTYPES = (torch.bfloat16, torch.float16)
@@ -48,7 +48,7 @@ class W4Weight:
     The constructor lays them out once in the tiles the kernels read (``swiglu_b200_w4_linear`` in the C header) and
     keeps only those; ``packed``, ``scales`` and ``zeros`` are rebuilt on request."""
 
-    __slots__ = ("tiles", "tile_scales", "tile_zeros", "out_features", "in_features", "group_size")
+    __slots__ = ("tiles", "tile_scales", "tile_zeros", "out_features", "in_features", "group_size", "_pointers")
 
     def __init__(self, packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, *,
                  in_features: int, group_size: int = 128):
@@ -81,6 +81,11 @@ class W4Weight:
         self.tiles = p.reshape(rows, 2, 8, cols, 4, 4, 4).permute(0, 3, 1, 2, 5, 4, 6).contiguous()
         self.tile_scales = self._tile_groups(scales)
         self.tile_zeros = None if zeros is None else self._tile_groups(zeros)
+        self._set_pointers()
+
+    def _set_pointers(self) -> None:
+        self._pointers = (self.tiles.data_ptr(), self.tile_scales.data_ptr(),
+                          None if self.tile_zeros is None else self.tile_zeros.data_ptr())
 
     def _groups(self) -> int:
         return _ceil(self.in_features, TILE_COLS) * (TILE_COLS // self.group_size)
@@ -136,11 +141,8 @@ class W4Weight:
         other.out_features, other.in_features, other.group_size = self.out_features, self.in_features, self.group_size
         other.tiles, other.tile_scales = moved, self.tile_scales.to(device)
         other.tile_zeros = None if self.tile_zeros is None else self.tile_zeros.to(device)
+        other._set_pointers()
         return other
-
-    def _pointers(self):
-        return (self.tiles.data_ptr(), self.tile_scales.data_ptr(),
-                None if self.tile_zeros is None else self.tile_zeros.data_ptr())
 
     def dequantize(self) -> torch.Tensor:
         """``[out_features, in_features]`` in the dtype of the scales: ``(code - zero) * scale`` rounded once."""
@@ -150,7 +152,7 @@ class W4Weight:
         out = torch.empty((n, k), dtype=self.dtype, device=self.device)
         _lib.check(
             "W4Weight.dequantize",
-            _lib.lib.swiglu_b200_w4_dequantize(out.data_ptr(), *self._pointers(), n, k, k, self.group_size,
+            _lib.lib.swiglu_b200_w4_dequantize(out.data_ptr(), *self._pointers, n, k, k, self.group_size,
                                                _DTYPE_CODE[self.dtype], self.device.index, _stream(self.device)),
         )
         return out
@@ -216,18 +218,19 @@ def _check_tokens(x: torch.Tensor, w: W4Weight, what: str) -> None:
 def w4_linear(x: torch.Tensor, weight: W4Weight) -> torch.Tensor:
     """``x W^T`` for ``x`` ``[..., in_features]`` of the weight's dtype."""
     _check_tokens(x, weight, "w4_linear")
-    n, k = weight.shape
-    x2 = _rows(x)
-    m = x2.shape[0]
+    n, k = weight.out_features, weight.in_features
+    m = x.numel() // k
     if m > MATVEC_ROWS:
-        return (x2 @ weight.dequantize().t()).view(*x.shape[:-1], n)
-    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+        return x @ weight.dequantize().t()
+    y = x.new_empty((*x.shape[:-1], n))
+    x, pitch = _rows(x)
+    device = x.device
     _lib.check(
         "w4_linear",
-        _lib.lib.swiglu_b200_w4_linear(y.data_ptr(), x2.data_ptr(), *weight._pointers(), m, n, k, _pitch(x2), n,
-                                       weight.group_size, _DTYPE_CODE[x.dtype], x.device.index, _stream(x.device)),
+        _lib.lib.swiglu_b200_w4_linear(y.data_ptr(), x.data_ptr(), *weight._pointers, m, n, k, pitch, n,
+                                       weight.group_size, _DTYPE_CODE[x.dtype], device.index, _stream(device)),
     )
-    return y.view(*x.shape[:-1], n)
+    return y
 
 
 def _gate_up_16bit(x, w_gate, w_up, activation, gm, dm):
@@ -254,25 +257,25 @@ def w4_gate_up(x: torch.Tensor, w_gate: W4Weight, w_up: W4Weight, activation: st
     on the way."""
     _check_activation(activation)
     gm, dm = _check_multipliers(activation, gate_multiplier, down_multiplier)
-    if w_gate.shape != w_up.shape or w_gate.group_size != w_up.group_size or w_gate.dtype != w_up.dtype:
-        raise ValueError("w_gate and w_up must agree in shape, group size and dtype")
+    if (w_gate.out_features != w_up.out_features or w_gate.in_features != w_up.in_features
+            or w_gate.group_size != w_up.group_size or w_gate.dtype != w_up.dtype or w_gate.device != w_up.device):
+        raise ValueError("w_gate and w_up must agree in shape, group size, dtype and device")
     _check_tokens(x, w_gate, "w4_gate_up")
-    _check_tokens(x, w_up, "w4_gate_up")
-    n, k = w_gate.shape
-    x2 = _rows(x)
-    m = x2.shape[0]
+    n, k = w_gate.out_features, w_gate.in_features
+    m = x.numel() // k
     if m > MATVEC_ROWS:
         return _gate_up_16bit(x, w_gate, w_up, activation, gm, dm)
-    h = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    h = x.new_empty((*x.shape[:-1], n))
+    x, pitch = _rows(x)
+    device = x.device
     _lib.check(
         "w4_gate_up",
         _lib.lib.swiglu_b200_w4_gate_up(
-            h.data_ptr(), x2.data_ptr(), *w_gate._pointers(), *w_up._pointers(), m, n, k, _pitch(x2), n,
-            w_gate.group_size, _DTYPE_CODE[x.dtype], ACTIVATIONS[activation], gm, dm, x.device.index,
-            _stream(x.device),
+            h.data_ptr(), x.data_ptr(), *w_gate._pointers, *w_up._pointers, m, n, k, pitch, n, w_gate.group_size,
+            _DTYPE_CODE[x.dtype], ACTIVATIONS[activation], gm, dm, device.index, _stream(device),
         ),
     )
-    return h.view(*x.shape[:-1], n)
+    return h
 
 
 def w4_mlp(x: torch.Tensor, w_gate: W4Weight, w_up: W4Weight, w_down: W4Weight,

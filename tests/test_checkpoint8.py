@@ -116,8 +116,11 @@ def test_refusals():
         geglu_ckpt8(a, b, "sigmoid")
     with pytest.raises(TypeError, match="fp16, bf16, and fp32"):
         ckpt8_forward(a.double(), b.double())
-    kept = Checkpoint8(torch.zeros(2, 4, 32, dtype=torch.int8), torch.ones(2, 4, 1, dtype=torch.uint8), (4, 8),
-                       torch.float32)
+    kept = Checkpoint8(torch.ones(Checkpoint8.size((4, 8)), dtype=torch.uint8), (4, 8), torch.float32)
+    with pytest.raises(ValueError, match="is 264 bytes"):
+        Checkpoint8(torch.ones(263, dtype=torch.uint8), (4, 8), torch.float32)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ckpt8_backward(torch.zeros(4, 8), kept)
     with pytest.raises(ValueError, match="does not match"):
         ckpt8_backward(torch.zeros(4, 9), kept)
     with pytest.raises(TypeError, match="dtype and device"):
@@ -160,10 +163,10 @@ def test_c_entries_refuse_bad_arguments_without_a_device():
 
 
 def test_dequantize_reads_the_codes_on_any_device():
-    codes = torch.zeros(2, 1, 32, dtype=torch.int8)
-    codes[0, 0, :3] = torch.tensor([127, -127, 1])
-    codes[1, 0, 0] = 5
-    kept = Checkpoint8(codes, torch.tensor([[[127]], [[255]]], dtype=torch.uint8), (3,), torch.float32)
+    kept = Checkpoint8(torch.zeros(66, dtype=torch.uint8), (3,), torch.float32)
+    kept.codes[0, 0, :3] = torch.tensor([127, -127, 1])
+    kept.codes[1, 0, 0] = 5
+    kept.steps[:] = torch.tensor([[[127]], [[255]]])
     g, u = kept.dequantize()
     assert g.tolist() == [127.0, -127.0, 1.0] and bool(torch.isnan(u).all())
     assert kept.nbytes == 66

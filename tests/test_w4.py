@@ -275,14 +275,14 @@ def test_pitched_and_misaligned_tokens(dtype, m, offset, extra):
     out = torch.full((16 + m * (n + 5),), 55.0, dtype=dtype, device="cuda")
     y = out[8:8 + m * (n + 5)].view(m, n + 5)[:, :n]
     st = torch.cuda.current_stream().cuda_stream
-    assert _lib.lib.swiglu_b200_w4_linear(y.data_ptr(), x.data_ptr(), *w._pointers(), m, n, k, k, n + 5, 64,
+    assert _lib.lib.swiglu_b200_w4_linear(y.data_ptr(), x.data_ptr(), *w._pointers, m, n, k, k, n + 5, 64,
                                           CODES[dtype], -1, st) == 0
     assert torch.equal(y, want)
     y.fill_(55.0)
     assert bool((out == 55.0).all())
     full = torch.full((n * (k + 7) + 16,), 55.0, dtype=dtype, device="cuda")
     d = full[5:5 + n * (k + 7)].view(n, k + 7)[:, :k]
-    assert _lib.lib.swiglu_b200_w4_dequantize(d.data_ptr(), *w._pointers(), n, k, k + 7, 64, CODES[dtype], -1, st) == 0
+    assert _lib.lib.swiglu_b200_w4_dequantize(d.data_ptr(), *w._pointers, n, k, k + 7, 64, CODES[dtype], -1, st) == 0
     assert torch.equal(d, w.dequantize())
     d.fill_(55.0)
     assert bool((full == 55.0).all())
