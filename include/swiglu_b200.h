@@ -341,28 +341,30 @@ SWIGLU_B200_API int swiglu_b200_ckpt8_bwd(void* h, void* dgate, void* dup, const
  *   gate_up   h = act(gm * (x . w_gate^T)) * (x . w_up^T) * dm, both projections in one launch
  * Sums and the scaling are fp32, the result is rounded once; gm, dm are ignored by the GELU activations.
  *
- * Weight layout, made once per weight.  q is cut into tiles of 16 rows x 128 columns, zero-padded to whole tiles, in
- * the order [row tile][column tile]; a tile is 1024 bytes, [hi 0..1][g 0..7][t 0..3][u 0..3] 32-bit words, and word
- * (hi, g, t, u) holds row 8*hi + g, columns 32*u + 8*t .. +7 of the tile, the lowest column in the lowest 4 bits.
- *   tiles    16-byte aligned
- *   scales   [row tile][group][g 0..7][hi 0..1] of the element type, `group` counting 128/group per column tile, zero
- *            past the matrix; 4-byte aligned
- *   zeros    uint8 in the layout of the scales, values 0..15, 2-byte aligned; NULL means 8 everywhere
- *   x        m x k, row stride x_row_stride; any alignment of the element type (16-byte aligned rows are fastest)
+ * Weight layout, made once per weight.  The matrix is cut into blocks of 16 rows x 128 columns, padded to whole blocks
+ * with codes and scales of zero, in the order [row tile][column tile], without gaps.  A block is
+ *   codes    1024 bytes, 32-bit words [hi 0..1][g 0..7][t 0..3][u 0..3]: word (hi, g, t, u) holds row 8*hi + g, columns
+ *            32*u + 8*t .. +7 of the block, column 2i of these in bits 4i .. 4i+3, column 2i + 1 in bits 16 + 4i ..
+ *            16 + 4i+3, i = 0..3
+ *   scales   [g 0..7][group 0..128/group-1][hi 0..1] of the element type
+ *   zeros    only if the matrix has them: uint8 in the order of the scales, values 0..15 (otherwise z is 8)
+ * and the arguments are
+ *   blocks   16-byte aligned; zeros != 0 when its blocks have zero points
+ *   x        m x k, row stride x_row_stride; 16-byte aligned rows (a stride that is a multiple of 8 when m > 1)
  *   y, h     m x n, row stride given; may not overlap x or the weights
  *   group    32, 64 or 128 columns share a scale
  * Meant for m up to a few tens: every 32 tokens read the weights again. */
-SWIGLU_B200_API int swiglu_b200_w4_linear(void* y, const void* x, const void* tiles, const void* scales, const void* zeros,
-                          int64_t m, int64_t n, int64_t k, int64_t x_row_stride, int64_t y_row_stride, int group,
-                          int dtype, int device, void* stream);
-SWIGLU_B200_API int swiglu_b200_w4_gate_up(void* h, const void* x, const void* gate_tiles, const void* gate_scales,
-                           const void* gate_zeros, const void* up_tiles, const void* up_scales, const void* up_zeros,
-                           int64_t m, int64_t n, int64_t k, int64_t x_row_stride, int64_t h_row_stride, int group,
-                           int dtype, int activation, float gm, float dm, int device, void* stream);
+SWIGLU_B200_API int swiglu_b200_w4_linear(void* y, const void* x, const void* blocks, int zeros, int64_t m, int64_t n,
+                          int64_t k, int64_t x_row_stride, int64_t y_row_stride, int group, int dtype, int device,
+                          void* stream);
+SWIGLU_B200_API int swiglu_b200_w4_gate_up(void* h, const void* x, const void* gate_blocks, int gate_zeros,
+                           const void* up_blocks, int up_zeros, int64_t m, int64_t n, int64_t k, int64_t x_row_stride,
+                           int64_t h_row_stride, int group, int dtype, int activation, float gm, float dm, int device,
+                           void* stream);
 
 /* A 4-bit weight written out: out[n][k] = (q - z) * s rounded once to the element type, row stride out_row_stride. */
-SWIGLU_B200_API int swiglu_b200_w4_dequantize(void* out, const void* tiles, const void* scales, const void* zeros, int64_t n,
-                              int64_t k, int64_t out_row_stride, int group, int dtype, int device, void* stream);
+SWIGLU_B200_API int swiglu_b200_w4_dequantize(void* out, const void* blocks, int zeros, int64_t n, int64_t k,
+                              int64_t out_row_stride, int group, int dtype, int device, void* stream);
 
 /* Number of fused-GEMM kernels launched by this process. */
 SWIGLU_B200_API uint64_t swiglu_b200_gemm_launch_count(void);

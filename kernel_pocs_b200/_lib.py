@@ -110,16 +110,16 @@ SIGNATURES = {
     ),
     "swiglu_b200_w4_linear": (
         ctypes.c_int,
-        [_c_ptr] * 5 + [_c_i64] * 5 + [ctypes.c_int, ctypes.c_int, ctypes.c_int, _c_ptr],
+        [_c_ptr] * 3 + [ctypes.c_int] + [_c_i64] * 5 + [ctypes.c_int, ctypes.c_int, ctypes.c_int, _c_ptr],
     ),
     "swiglu_b200_w4_gate_up": (
         ctypes.c_int,
-        [_c_ptr] * 8 + [_c_i64] * 5 + [ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_float,
-                                       ctypes.c_int, _c_ptr],
+        [_c_ptr] * 3 + [ctypes.c_int, _c_ptr, ctypes.c_int] + [_c_i64] * 5 +
+        [ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_float, ctypes.c_int, _c_ptr],
     ),
     "swiglu_b200_w4_dequantize": (
         ctypes.c_int,
-        [_c_ptr] * 4 + [_c_i64] * 3 + [ctypes.c_int, ctypes.c_int, ctypes.c_int, _c_ptr],
+        [_c_ptr] * 2 + [ctypes.c_int] + [_c_i64] * 3 + [ctypes.c_int, ctypes.c_int, ctypes.c_int, _c_ptr],
     ),
     "swiglu_b200_gemm_bwd_launch_count": (ctypes.c_uint64, []),
     "swiglu_b200_selftest_wait_timeout": (

@@ -11,13 +11,15 @@
 // (fp16), and an exact subtraction of that plus the zero point.  q - z is exact in either type; the sum over a group is
 // a fp32 accumulator which is multiplied by the group's scale in fp32: nothing is rounded to 16 bits before the result.
 //
-// Weight tiles.  The fragments fix which lane needs which nibbles, so weights are laid out once for it: 16 rows x 128
+// Weight blocks.  The fragments fix which lane needs which nibbles, so weights are laid out once for it: 16 rows x 128
 // columns are 1 KB in which lane l = 4g + t finds the 32 nibbles of row g (and, 512 bytes on, of row g + 8) that it
-// feeds to the tile's eight instructions, as one 16-byte load; a warp's load is 512 contiguous bytes and the tiles of a
-// row are contiguous along k.  Word u of a lane holds columns 32u + 8t .. +7, so the 4 lanes of a row cover 32 columns
-// with each word and a group of 32 never mixes with the next inside one instruction.
+// feeds to the block's instructions, as one 16-byte load.  Word u of a lane holds columns 32u + 8t .. +7, so the 4 lanes
+// of a row cover 32 columns with each word and a group of 32 never mixes with the next inside one instruction.  The
+// scales (and zero points) of those rows and columns follow the codes, and the blocks of 16 rows are contiguous along k:
+// a warp reads one stream, whatever the group size.
 #include "swiglu_b200.h"
 
+#include <atomic>
 #include <type_traits>
 
 #include "launch_common.cuh"
@@ -30,26 +32,37 @@ using namespace swiglu_b200;
 constexpr int kTileRows = 16, kTileCols = 128, kTileBytes = kTileRows * kTileCols / 2;
 constexpr int kWarps = 8;
 
-// One 4-bit weight matrix in tiles.
+// One 4-bit weight matrix in blocks.
 struct W4 {
-  const void* tiles;   // [row tiles][column tiles][2][32][16 bytes]
-  const void* scales;  // [row tiles][groups][8][2], rows g and g + 8 side by side
-  const void* zeros;   // uint8, laid out as the scales; NULL means 8 everywhere
+  const void* blocks;  // [row tiles][column tiles]: codes, scales [8][groups][2], zero points likewise in bytes
+  int zeros;           // whether blocks have zero points; else they are 8
 };
+
+// Bytes of a block.
+__host__ __device__ constexpr int block_bytes(int groups, bool zeros) {
+  return kTileBytes + groups * 32 + (zeros ? groups * 16 : 0);
+}
 
 struct W4Shape {
   long long m, n, k;
   long long x_pitch, y_pitch;  // elements
   int col_tiles;
   int groups_log2;  // log2 of the groups per column tile (0, 1, 2)
-  int x_vec;        // every row of x starts on a 16-byte boundary
+  int split;        // CTAs that share a row of column tiles, a cluster
 };
 
 template <class T> struct Half2;
 template <> struct Half2<__nv_bfloat16> {
   using V = __nv_bfloat162;
-  static constexpr uint32_t kMagic = 0x43004300u;  // (128, 128): one step of the mantissa is 1
-  static __device__ __forceinline__ uint32_t magic_plus(uint32_t z) { return kMagic + z * 0x00010001u; }
+  // A nibble in the low byte of a 16-bit number is that integer times 2^-133 (bf16), wherever it sits in the byte: the
+  // subnormals and the first binade go on in equal steps.  One multiply-add brings both places to the same unit and
+  // takes the zero point off; all of it is exact.
+  static constexpr uint32_t kLow = 0x7f007f00u, kHigh = 0x7d007d00u;  // 2^127, 2^123
+  static constexpr float kUnit = 0x1p-6f;
+  static __device__ __forceinline__ uint32_t pair(float f) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(f, f);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
   static __device__ __forceinline__ float to_float(uint32_t half_word) { return __uint_as_float(half_word << 16); }
   static __device__ __forceinline__ uint16_t from_float(float f) { return __bfloat16_as_ushort(__float2bfloat16_rn(f)); }
   static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -60,8 +73,12 @@ template <> struct Half2<__nv_bfloat16> {
 };
 template <> struct Half2<__half> {
   using V = __half2;
-  static constexpr uint32_t kMagic = 0x64006400u;  // (1024, 1024)
-  static __device__ __forceinline__ uint32_t magic_plus(uint32_t z) { return kMagic + z * 0x00010001u; }
+  static constexpr uint32_t kLow = 0x78007800u, kHigh = 0x68006800u;  // 2^15, 2^11; the step of the subnormals is 2^-24
+  static constexpr float kUnit = 0x1p-9f;
+  static __device__ __forceinline__ uint32_t pair(float f) {
+    __half2 v = __floats2half2_rn(f, f);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
   static __device__ __forceinline__ float to_float(uint32_t half_word) {
     return __half2float(__ushort_as_half((unsigned short)half_word));
   }
@@ -73,133 +90,548 @@ template <> struct Half2<__half> {
   }
 };
 
-// Nibbles I and I + 4 of a word as a pair of exact 16-bit numbers q - z.
-template <class T, int I>
-__device__ __forceinline__ uint32_t weight_pair(uint32_t word, uint32_t bias) {
-  using V = typename Half2<T>::V;
-  uint32_t w = ((word >> (4 * I)) & 0x000f000fu) | Half2<T>::kMagic;
-  V r = __hsub2(*reinterpret_cast<V*>(&w), *reinterpret_cast<V*>(&bias));
-  return *reinterpret_cast<uint32_t*>(&r);
-}
-
-// Columns k .. k+7 of a row of x, zero past column K.
+// Columns (2i, 2i+1) of a word, i = 0..3, as pairs of (q - z) * kUnit; `bias` is the pair -z * kUnit.
 template <class T>
-__device__ __forceinline__ Vec<16> x_load(const char* row, long long k, long long K, bool vec) {
-  if (vec && k + 8 <= K) return Ld<16, LD_PLAIN>::ld(row + k * 2);
-  Vec<16> v{};
+__device__ __forceinline__ void weight_pairs(uint32_t word, uint32_t bias, uint32_t (&p)[4]) {
+  using H = Half2<T>;
+  using V = typename H::V;
+  const uint32_t high = word >> 8;
+  const uint32_t raw[4] = {word & 0x000f000fu, word & 0x00f000f0u, high & 0x000f000fu, high & 0x00f000f0u};
+  const uint32_t low_unit = H::kLow, high_unit = H::kHigh;
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (k + e < K) v.w[e / 2] |= Ld<2, LD_PLAIN>::ld(row + (k + e) * 2).w[0] << (16 * (e & 1));
-  return v;
+  for (int i = 0; i < 4; ++i) {
+    V r = __hfma2(*reinterpret_cast<const V*>(&raw[i]),
+                  *reinterpret_cast<const V*>(i & 1 ? &high_unit : &low_unit), *reinterpret_cast<V*>(&bias));
+    p[i] = *reinterpret_cast<uint32_t*>(&r);
+  }
 }
 
-// A CTA owns RT row tiles of MATS matrices and NT * 8 tokens; its warps share the column tiles among them and add
-// their sums up in shared memory.
-template <class T, int MATS, int RT, int NT, int ACT>
-__global__ void __launch_bounds__(32 * kWarps)
-w4_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, float gm, float dm) {
+// A zero point 0..15 as a float.
+__device__ __forceinline__ float zero_point(uint32_t z) { return __uint_as_float(0x4b000000u | z) - 8388608.0f; }
+
+// Copies from global to shared memory in the calling thread's current group of copies.  copy16 goes past L1 and writes
+// zeros behind the first `bytes` bytes, which are all it reads.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes = 16) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void copies_wait() {  // until at most LEFT groups are in flight
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
+// The `bytes` (a multiple of 16) at `src`, copied by the calling warp; ROUNDS * 512 is at least the largest size.
+template <int ROUNDS>
+__device__ __forceinline__ void warp_copy(uint32_t dst, const char* src, int bytes, int lane) {
+#pragma unroll
+  for (int i = 0; i < ROUNDS; ++i)
+    if ((i * 32 + lane) * 16 < bytes) copy16(dst + (i * 32 + lane) * 16, src + (i * 32 + lane) * 16);
+}
+
+// Clusters.  A launch without one is a cluster of one CTA.
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_index() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+// Stores v at `addr` of the shared memory of CTA `rank` of the cluster.
+__device__ __forceinline__ void cluster_store(uint32_t addr, uint32_t rank, float v) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
+}
+
+// What a pair of projections (or one alone) comes to.
+template <int MATS>
+__device__ __forceinline__ float result(const float (&v)[MATS], int activation, const Consts& c) {
+  if constexpr (MATS == 1) return v[0];
+  else if (activation == ACT_SILU) return Math<true, ACT_SILU>::fwd(v[0], v[1], c);
+  else if (activation == ACT_GELU_TANH) return Math<true, ACT_GELU_TANH>::fwd(v[0], v[1], c);
+  else return Math<true, ACT_GELU_ERF>::fwd(v[0], v[1], c);
+}
+
+constexpr int kTokenBytes = kTileCols * 2;  // a token's part of a column tile
+
+// ------------------------------------------------------------------ up to 32 tokens: 16-bit products
+
+// Shared memory of a CTA: DEPTH stages of one column tile each, then where the cluster's sums arrive.
+template <int MATS, int RT, int NT, int GROUPS> struct Cfg {
+  static constexpr int SLOT = block_bytes(GROUPS, true);
+  static constexpr int WEIGHTS = kWarps * MATS * RT * SLOT, STAGE = WEIGHTS + 8 * NT * kTokenBytes;
+  static constexpr int CTAS = MATS * RT * NT == 1 ? 3 : 2;  // to an SM
+  static constexpr int OUTPUTS = kWarps * RT * kTileRows * 8 * NT;
+  static constexpr int ARRIVALS = MATS * (OUTPUTS + 64) * 4;
+  static constexpr int FIT = (220 * 1024 / CTAS - ARRIVALS) / STAGE;
+  static constexpr int DEPTH = FIT < 3 ? 3 : FIT > 8 ? 8 : FIT;
+  static constexpr int SMEM = DEPTH * STAGE + ARRIVALS;
+  static_assert(kWarps * MATS * RT * NT * 4 * 32 * 4 <= DEPTH * STAGE, "the sums on their way out reuse the stages");
+};
+
+// A CTA owns 8 * RT row tiles (RT to a warp) of MATS matrices, 8 * NT tokens and, as rank r of a cluster of `split`
+// CTAs, the r-th part of the column tiles.  Each rank finishes a slice of the outputs: the others store their sums for
+// it into its shared memory, where they are added in a fixed order.
+template <class T, int MATS, int RT, int NT, int GROUPS>
+__global__ void __launch_bounds__(32 * kWarps, Cfg<MATS, RT, NT, GROUPS>::CTAS)
+w4_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, int activation, float gm, float dm) {
   using H = Half2<T>;
-  __shared__ float red[kWarps][MATS * RT * NT * 4][32];
+  using C = Cfg<MATS, RT, NT, GROUPS>;
+  constexpr int DEPTH = C::DEPTH, PIECES = 8 * NT * 16, ROUNDS = (PIECES + 32 * kWarps - 1) / (32 * kWarps);
+  extern __shared__ __align__(16) unsigned char smem[];
+  cluster_arrive();  // all CTAs of the cluster have started once this is waited for
+  const uint32_t smem_addr = (uint32_t)__cvta_generic_to_shared(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const long long row_tile = (long long)blockIdx.x * RT, row_tiles = (s.n + kTileRows - 1) / kTileRows;
+  const int rank = (int)cluster_rank(), split = s.split;
+  const int row_tiles = (int)((s.n + kTileRows - 1) / kTileRows);
+  const int row_tile0 = (int)cluster_index() * (kWarps * RT), row_tile = row_tile0 + warp * RT;  // of the CTA, the warp
   const long long token0 = (long long)blockIdx.y * (8 * NT);
+  const int share = s.col_tiles / split, over = s.col_tiles % split;
+  const int first = rank * share + min(rank, over), last = first + share + (rank < over ? 1 : 0);
   const W4 w[2] = {w0, w1};
 
-  float acc[MATS][RT][NT][4] = {};
-  for (int c = warp; c < s.col_tiles; c += kWarps) {
-    Vec<16> q[MATS][RT][2];
+  const char* src[MATS][RT];  // the warp's next block of each row tile
 #pragma unroll
-    for (int i = 0; i < MATS; ++i)
+  for (int a = 0; a < MATS; ++a)
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        const bool there = row_tile + r < row_tiles;
-        const char* p = cbyte(w[i].tiles) + ((row_tile + r) * s.col_tiles + c) * kTileBytes + lane * 16;
+    for (int r = 0; r < RT; ++r)
+      src[a][r] = cbyte(w[a].blocks) + ((long long)(row_tile + r) * s.col_tiles + first) * block_bytes(GROUPS, w[a].zeros);
+  const char* x_src[ROUNDS];  // this thread's pieces of 8 columns of a token, and how many bytes of the row are left there
+  long long x_left[ROUNDS];
 #pragma unroll
-        for (int hi = 0; hi < 2; ++hi) q[i][r][hi] = there ? Ld<16, LD_NC_NOALLOC>::ld(p + hi * 512) : Vec<16>{};
+  for (int i = 0; i < ROUNDS; ++i) {
+    const int o = threadIdx.x + i * 32 * kWarps, tok = o >> 4, piece = o & 15;
+    const long long k = (long long)first * kTileCols + 8 * piece;
+    const bool mine = o < PIECES && token0 + tok < s.m;
+    x_src[i] = mine ? cbyte(x) + ((token0 + tok) * s.x_pitch + k) * 2 : cbyte(x);
+    x_left[i] = mine ? (s.k - k) * 2 : 0;
+  }
+  int fill = 0;  // offset of the stage to fill next
+  // Starts the copies of column tile c; always one group, empty past the last tile.
+  auto fetch = [&](int c) {
+    if (c < last) {
+      const uint32_t stage = smem_addr + fill;
+#pragma unroll
+      for (int a = 0; a < MATS; ++a)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const int bytes = block_bytes(GROUPS, w[a].zeros);
+          if (row_tile + r < row_tiles)
+            warp_copy<(C::SLOT + 511) / 512>(stage + ((warp * MATS + a) * RT + r) * C::SLOT, src[a][r], bytes, lane);
+          src[a][r] += bytes;
+        }
+      // tokens: every other one has its 64-byte quarters swapped in pairs, so that the 8 lanes that read together (two
+      // tokens, four pieces) touch all 32 banks
+#pragma unroll
+      for (int i = 0; i < ROUNDS; ++i) {
+        const int o = threadIdx.x + i * 32 * kWarps, tok = o >> 4, piece = o & 15;
+        if (PIECES % (32 * kWarps) == 0 || o < PIECES)
+          copy16(stage + C::WEIGHTS + tok * kTokenBytes + (piece ^ ((tok & 1) << 2)) * 16, x_left[i] > 0 ? x_src[i] : cbyte(x),
+                 x_left[i] >= 16 ? 16u : x_left[i] > 0 ? (uint32_t)x_left[i] : 0u);
+        x_src[i] += kTokenBytes;
+        x_left[i] -= kTokenBytes;
       }
-    Vec<16> b[NT][4];
+    }
+    copies_commit();
+    fill = fill == (DEPTH - 1) * C::STAGE ? 0 : fill + C::STAGE;
+  };
+
+#pragma unroll 1
+  for (int i = 0; i < DEPTH - 1; ++i) fetch(first + i);
+
+  float acc[MATS][RT][NT][4] = {};
+  int take = 0;  // offset of the stage to read next
+#pragma unroll 1
+  for (int c = first; c < last; ++c) {
+    copies_wait<DEPTH - 2>();
+    __syncthreads();  // this stage is there for all, and the one before has been read by all
+    fetch(c + DEPTH - 1);
+    const unsigned char* stage = smem + take;
+    take = take == (DEPTH - 1) * C::STAGE ? 0 : take + C::STAGE;
+    uint4 b[NT][4];  // columns 32u + 8t .. +7 of the tokens, in the pairs that a weight word comes apart into
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const long long token = token0 + j * 8 + g;
-      const char* row = cbyte(x) + token * s.x_pitch * 2;
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        b[j][u] = token < s.m ? x_load<T>(row, (long long)c * kTileCols + 32 * u + 8 * t, s.k, s.x_vec) : Vec<16>{};
-    }
+        b[j][u] = *reinterpret_cast<const uint4*>(stage + C::WEIGHTS + (8 * j + g) * kTokenBytes +
+                                                  ((4 * u + t) ^ ((g & 1) << 2)) * 16);
 #pragma unroll
-    for (int i = 0; i < MATS; ++i)
+    for (int a = 0; a < MATS; ++a)
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
         if (row_tile + r >= row_tiles) continue;
-        const long long group0 = ((row_tile + r) * s.col_tiles + c) << s.groups_log2;
-        float part[NT][4] = {};
+        const unsigned char* slot = stage + ((warp * MATS + a) * RT + r) * C::SLOT;
+        const uint4 lo4 = *reinterpret_cast<const uint4*>(slot + lane * 16);
+        const uint4 hi4 = *reinterpret_cast<const uint4*>(slot + 512 + lane * 16);
+        const uint32_t lo[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, hi[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
+        float part[NT][4];
         uint32_t bias_lo = 0, bias_hi = 0;
-        float scale_lo = 0, scale_hi = 0;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const int per_group = 4 >> s.groups_log2;  // words per group
+          constexpr int per_group = 4 / GROUPS;  // words per group
+          const int at = (g * GROUPS + u / per_group) * 2;
           if (u % per_group == 0) {
-            const long long at = (group0 + u / per_group) * 16 + 2 * g;
-            const uint32_t sc = Ld<4, LD_PLAIN>::ld(cbyte(w[i].scales) + at * 2).w[0];
-            scale_lo = H::to_float(sc & 0xffffu);
-            scale_hi = H::to_float(sc >> 16);
-            const uint32_t z = w[i].zeros ? Ld<2, LD_PLAIN>::ld(cbyte(w[i].zeros) + at).w[0] : 0x0808u;
-            bias_lo = H::magic_plus(z & 0xffu);
-            bias_hi = H::magic_plus(z >> 8);
+            bias_lo = bias_hi = H::pair(-8.0f * H::kUnit);
+            if (w[a].zeros) {
+              const uint32_t z = *reinterpret_cast<const uint16_t*>(slot + kTileBytes + GROUPS * 32 + at);
+              bias_lo = H::pair(-H::kUnit * zero_point(z & 0xffu));
+              bias_hi = H::pair(-H::kUnit * zero_point(z >> 8));
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) part[j][0] = part[j][1] = part[j][2] = part[j][3] = 0.0f;
           }
-          const uint32_t lo = q[i][r][0].w[u], hi = q[i][r][1].w[u];
-          const uint32_t a0[4] = {weight_pair<T, 0>(lo, bias_lo), weight_pair<T, 0>(hi, bias_hi),
-                                  weight_pair<T, 1>(lo, bias_lo), weight_pair<T, 1>(hi, bias_hi)};
-          const uint32_t a1[4] = {weight_pair<T, 2>(lo, bias_lo), weight_pair<T, 2>(hi, bias_hi),
-                                  weight_pair<T, 3>(lo, bias_lo), weight_pair<T, 3>(hi, bias_hi)};
+          uint32_t wl[4], wh[4];
+          weight_pairs<T>(lo[u], bias_lo, wl);
+          weight_pairs<T>(hi[u], bias_hi, wh);
+          const uint32_t a0[4] = {wl[0], wh[0], wl[1], wh[1]}, a1[4] = {wl[2], wh[2], wl[3], wh[3]};
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            const uint32_t* xw = b[j][u].w;  // columns (0,1) (2,3) (4,5) (6,7) of the lane's eight
-            H::mma(part[j], a0, __byte_perm(xw[0], xw[2], 0x5410), __byte_perm(xw[0], xw[2], 0x7632));
-            H::mma(part[j], a1, __byte_perm(xw[1], xw[3], 0x5410), __byte_perm(xw[1], xw[3], 0x7632));
+            H::mma(part[j], a0, b[j][u].x, b[j][u].y);
+            H::mma(part[j], a1, b[j][u].z, b[j][u].w);
           }
           if ((u + 1) % per_group == 0) {
+            const uint32_t sc = *reinterpret_cast<const uint32_t*>(slot + kTileBytes + at * 2);
+            const float scale_lo = H::to_float(sc & 0xffffu), scale_hi = H::to_float(sc >> 16);
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-              acc[i][r][j][0] = fmaf(part[j][0], scale_lo, acc[i][r][j][0]);
-              acc[i][r][j][1] = fmaf(part[j][1], scale_lo, acc[i][r][j][1]);
-              acc[i][r][j][2] = fmaf(part[j][2], scale_hi, acc[i][r][j][2]);
-              acc[i][r][j][3] = fmaf(part[j][3], scale_hi, acc[i][r][j][3]);
-              part[j][0] = part[j][1] = part[j][2] = part[j][3] = 0.0f;
+              acc[a][r][j][0] = fmaf(part[j][0], scale_lo, acc[a][r][j][0]);
+              acc[a][r][j][1] = fmaf(part[j][1], scale_lo, acc[a][r][j][1]);
+              acc[a][r][j][2] = fmaf(part[j][2], scale_hi, acc[a][r][j][2]);
+              acc[a][r][j][3] = fmaf(part[j][3], scale_hi, acc[a][r][j][3]);
             }
           }
         }
       }
   }
 
+  copies_wait<0>();
+  __syncthreads();  // the stages are done with
+  constexpr int kRows = kWarps * RT * kTileRows, OUTPUTS = C::OUTPUTS;
+  float* sums = reinterpret_cast<float*>(smem);  // [matrix][token][row]
 #pragma unroll
-  for (int i = 0; i < MATS; ++i)
+  for (int a = 0; a < MATS; ++a)
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) red[warp][((i * RT + r) * NT + j) * 4 + e][lane] = acc[i][r][j][e];
+        for (int e = 0; e < 4; ++e)  // row g + 8 (e / 2), token 2t + e % 2 of a tile
+          sums[a * OUTPUTS + (8 * j + 2 * t + e % 2) * kRows + (warp * RT + r) * kTileRows + g + 8 * (e / 2)] =
+              acc[a][r][j][e] * (1.0f / H::kUnit);
   __syncthreads();
 
+  // The part of the outputs [token][row] that exist; each rank finishes `slice` of them.
+  const int tokens = s.m - token0 < 8 * NT ? (int)(s.m - token0) : 8 * NT, outputs = tokens * kRows;
+  const int slice = (outputs + split - 1) / split;
+  const float* parts = sums;
+  int part_pitch = 0, begin = 0;
+  if (split > 1) {
+    const uint32_t arrivals = smem_addr + DEPTH * C::STAGE;  // [matrix][rank][slice]
+    cluster_wait();
+#pragma unroll 1
+    for (int o = threadIdx.x; o < outputs; o += 32 * kWarps) {
+      const int owner = o / slice, at = rank * slice + o - owner * slice;
+#pragma unroll
+      for (int a = 0; a < MATS; ++a) cluster_store(arrivals + (a * (OUTPUTS + 64) + at) * 4, owner, sums[a * OUTPUTS + o]);
+    }
+    cluster_arrive();
+    parts = reinterpret_cast<const float*>(smem + DEPTH * C::STAGE);
+    part_pitch = slice;
+    begin = rank * slice;
+  }
+  cluster_wait();
   const Consts consts(gm, dm);
-  for (int o = threadIdx.x; o < RT * kTileRows * NT * 8; o += 32 * kWarps) {
-    const int row = o % (RT * kTileRows), tok = o / (RT * kTileRows);
-    const long long n = row_tile * kTileRows + row, token = token0 + tok;
-    if (n >= s.n || token >= s.m) continue;
-    // where lane 4g + t keeps (row g + 8 hi, token 2t + lo) of a tile
-    const int r = row / kTileRows, hi = row / 8 % 2, slot = (row % 8) * 4 + tok % 8 / 2;
+#pragma unroll 1
+  for (int o = threadIdx.x; o < slice && begin + o < outputs; o += 32 * kWarps) {
+    const int row = (begin + o) % kRows, tok = (begin + o) / kRows;
+    const long long n = (long long)row_tile0 * kTileRows + row;
+    if (n >= s.n) continue;
     float v[MATS];
 #pragma unroll
-    for (int i = 0; i < MATS; ++i) {
-      const int at = ((i * RT + r) * NT + tok / 8) * 4 + 2 * hi + tok % 2;
-      v[i] = 0.0f;
-#pragma unroll
-      for (int p = 0; p < kWarps; ++p) v[i] += red[p][at][slot];
+    for (int a = 0; a < MATS; ++a) {
+      const float* p = parts + a * (split > 1 ? OUTPUTS + 64 : OUTPUTS) + o;
+      v[a] = p[0];
+#pragma unroll 1
+      for (int i = 1; i < split; ++i) v[a] += p[i * part_pitch];
     }
-    float out = v[0];
-    if constexpr (MATS == 2) out = Math<true, ACT>::fwd(v[0], v[1], consts);
-    static_cast<uint16_t*>(y)[token * s.y_pitch + n] = H::from_float(out);
+    static_cast<uint16_t*>(y)[(token0 + tok) * s.y_pitch + n] = H::from_float(result<MATS>(v, activation, consts));
+  }
+}
+
+// ------------------------------------------------------------------ one or two tokens: digits and integer products
+
+// As bytes the 8 nibbles of a word are two registers after three instructions (9 and four multiply-adds above), and
+// m16n8k32 multiplies them as they are.  For that a token is written as three 8-bit digits of a 23-bit number: with
+// 2^e above the largest magnitude of its 256 columns, X = rint(x * 2^(22-e)) = d0 + 2^8 d1 + 2^16 d2, the digits
+// balanced around zero.  Its digits are three columns of the product, so two tokens fill the eight columns of one
+// instruction.  Within a group the sums of nibble * digit are exact in 32 bits, the zero point comes off as z times the
+// digits' own sum (exact as well), and what is left, below 2^19, goes on in fp32: times the group's scale and 2^(8i+e-22).
+// A column is thus rounded by at most 2^-23 of the largest one beside it, which is what summing in fp32 does to it;
+// 16-bit numbers within 2^12 (fp16) or 2^15 (bf16) of the largest are exact.  A token with an Inf or a NaN gives NaN.
+
+constexpr int kDigitTokens = 2, kDigitCols = 3 * kDigitTokens;
+constexpr int kSlab = 16;                              // column tiles whose digits are kept at a time, in pairs
+constexpr int kRowWarps = 4, kColWarps = kWarps / kRowWarps;  // a CTA: four row tiles, the tile pairs dealt to two warps
+
+constexpr int kDigitOutputs = kRowWarps * kTileRows * kDigitTokens;
+
+template <int MATS, int GROUPS> struct DigitCfg {
+  static constexpr int SLOT = 2 * block_bytes(GROUPS, true);      // a pair of blocks
+  static constexpr int PAIR = MATS * SLOT;
+  static constexpr int DEPTH = MATS == 1 ? 3 : 2;                 // pairs of a warp in flight
+  static constexpr int RING = kWarps * DEPTH * PAIR;
+  static constexpr int DIGITS = kSlab * 2 * kDigitCols * 4 * 16;  // [tile][2][column][t] 16 bytes
+  static constexpr int SUMS = kSlab * GROUPS * 8 * 4;             // [tile][group][8]
+  static constexpr int UNITS = kSlab / 2 * 8 * 4;                 // [pair][8]
+  static constexpr int ARRIVALS = MATS * kColWarps * (kDigitOutputs + 64) * 4;  // [matrix][column warp][rank][slice]
+  static constexpr int SMEM = RING + DIGITS + SUMS + UNITS + ARRIVALS;
+};
+
+__device__ __forceinline__ void imma(uint32_t (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                     uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Largest magnitude of eight 16-bit numbers as the bit pattern of a float.
+template <class T> __device__ __forceinline__ uint32_t top_of(const Vec<16>& v);
+template <> __device__ __forceinline__ uint32_t top_of<__nv_bfloat16>(const Vec<16>& v) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = max(m, max(v.w[i] << 16 & 0x7fffffffu, v.w[i] & 0x7fff0000u));
+  return m;
+}
+template <> __device__ __forceinline__ uint32_t top_of<__half>(const Vec<16>& v) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = max(m, max(v.w[i] & 0x7fffu, v.w[i] >> 16 & 0x7fffu));
+  return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+}
+
+constexpr float kIntMagic = 12582912.0f;  // 1.5 * 2^23: added to an integer below 2^22, its bits are 0x4b400000 + it
+constexpr uint32_t kIntMagicBits = 0x4b400000u;
+
+// A CTA owns kRowWarps row tiles of MATS matrices, up to two tokens and, as rank r of a cluster of `split` CTAs, the
+// r-th part of the pairs of column tiles.  The code is kept short (loops that are not unrolled): a launch lasts a few
+// microseconds, most of its instructions run once, and a start waits for them to be fetched.
+template <class T, int MATS, int GROUPS>
+__global__ void __launch_bounds__(32 * kWarps, 3)
+w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, int activation, float gm, float dm) {
+  using H = Half2<T>;
+  using C = DigitCfg<MATS, GROUPS>;
+  constexpr int DEPTH = C::DEPTH;
+  extern __shared__ __align__(16) unsigned char smem[];
+  cluster_arrive();  // all CTAs of the cluster have started once this is waited for
+  const uint32_t smem_addr = (uint32_t)__cvta_generic_to_shared(smem);
+  unsigned char* digits = smem + C::RING;
+  float* digit_sums = reinterpret_cast<float*>(digits + C::DIGITS);
+  float* units = reinterpret_cast<float*>(digits + C::DIGITS + C::SUMS);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int row_warp = warp % kRowWarps, col_warp = warp / kRowWarps;
+  const int rank = (int)cluster_rank(), split = s.split;
+  const int pairs = (s.col_tiles + 1) / 2, share = pairs / split, over = pairs % split;
+  const int first = rank * share + min(rank, over), last = first + share + (rank < over ? 1 : 0);
+  const int row_tile0 = (int)cluster_index() * kRowWarps, row_tile = row_tile0 + row_warp;  // of the CTA, the warp
+  const bool there = (long long)row_tile * kTileRows < s.n;
+  const long long token0 = (long long)blockIdx.y * kDigitTokens;
+  const int tokens = s.m - token0 < kDigitTokens ? (int)(s.m - token0) : kDigitTokens;
+  const W4 w[2] = {w0, w1};
+
+  // This thread's eight columns of a token, of the slab that starts at pair p.
+  auto read_token = [&](int p, int tok) {
+    const long long k = (long long)p * (2 * kTileCols) + 8 * threadIdx.x;
+    const char* src = cbyte(x) + ((token0 + tok) * s.x_pitch + k) * 2;
+    Vec<16> v{};
+    if (k + 8 <= s.k) {
+      v = Ld<16, LD_PLAIN>::ld(src);
+    } else {
+#pragma unroll 1
+      for (int e = 0; k + e < s.k; ++e) {
+        const uint32_t bits = Ld<2, LD_PLAIN>::ld(src + 2 * e).w[0] << (16 * (e & 1));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v.w[i] |= e / 2 == i ? bits : 0u;
+      }
+    }
+    return v;
+  };
+  // Writes its digits, and what goes with them.
+  auto write_digits = [&](const Vec<16>& v, int tok) {
+    const int piece = threadIdx.x & 15, tile = threadIdx.x >> 4, u = piece >> 2;
+    const int e = (int)(__reduce_max_sync(0xffffffffu, top_of<T>(v)) >> 23);  // the magnitudes are below 2^(e - 126)
+    if (lane < 3) units[warp * 8 + 3 * tok + lane] = e == 255 ? __uint_as_float(0x7fffffffu) : ldexpf(1.0f, e - 148 + 8 * lane);
+    const int up = 148 - e, half = up >> 1;  // 2^up as a product of two floats
+    const float f1 = __uint_as_float((uint32_t)(half + 127) << 23), f2 = __uint_as_float((uint32_t)(up - half + 127) << 23);
+    float f[8];
+    Codec<T>::template unpack<16>(v, f);
+    uint32_t z[8];  // bytes 0, 1, 2: the digits
+#pragma unroll
+    for (int a = 0; a < 8; ++a)
+      z[a] = (__float_as_uint(fmaf(f[a] * f1, f2, kIntMagic)) + (0x8080u - kIntMagicBits)) ^ 0x8080u;
+    int total[3];
+#pragma unroll
+    for (int d = 0; d < 3; ++d) {
+      // in the order of the nibbles: even ones columns 0, 4, 1, 5, odd ones 2, 6, 3, 7
+      const uint32_t pick = d | (4 + d) << 4;
+      const uint32_t even = __byte_perm(__byte_perm(z[0], z[4], pick), __byte_perm(z[1], z[5], pick), 0x5410);
+      const uint32_t odd = __byte_perm(__byte_perm(z[2], z[6], pick), __byte_perm(z[3], z[7], pick), 0x5410);
+      total[d] = __dp4a((int)even, 0x01010101, __dp4a((int)odd, 0x01010101, 0));
+      *reinterpret_cast<uint2*>(digits + (((tile * 2 + (u >> 1)) * kDigitCols + 3 * tok + d) * 4 + (piece & 3)) * 16 +
+                                (u & 1) * 8) = make_uint2(even, odd);
+    }
+    // sums over the 4, 8 or 16 threads of a group; two of them travel in one register (each below 2^15)
+    int both = total[0] + (total[1] << 16);
+#pragma unroll
+    for (int d = 1; d < 16 / GROUPS; d *= 2) {
+      both += __shfl_xor_sync(0xffffffffu, both, d);
+      total[2] += __shfl_xor_sync(0xffffffffu, total[2], d);
+    }
+    if (piece % (16 / GROUPS) == 0) {
+      float* to = digit_sums + (threadIdx.x / (16 / GROUPS)) * 8 + 3 * tok;
+      to[0] = (float)(short)both;
+      to[1] = (float)((both - (short)both) >> 16);
+      to[2] = (float)total[2];
+    }
+  };
+
+  // The warp's ring of pairs of blocks.
+  const unsigned char* ring = smem + warp * (DEPTH * C::PAIR);
+  const uint32_t ring_addr = smem_addr + warp * (DEPTH * C::PAIR);
+  const char* src[MATS];  // the warp's next pair
+#pragma unroll
+  for (int a = 0; a < MATS; ++a)
+    src[a] = cbyte(w[a].blocks) +
+             ((long long)row_tile * s.col_tiles + 2 * (first + col_warp)) * block_bytes(GROUPS, w[a].zeros);
+  int fill = 0;  // offset of the slot to fill next
+  auto fetch = [&](int p) {  // always one group of copies, empty past the last pair
+    if (p < last && there) {
+#pragma unroll
+      for (int a = 0; a < MATS; ++a) {
+        const int bytes = block_bytes(GROUPS, w[a].zeros);
+        warp_copy<(C::SLOT + 511) / 512>(ring_addr + fill + a * C::SLOT, src[a], 2 * p + 1 == s.col_tiles ? bytes : 2 * bytes,
+                                         lane);
+        src[a] += 2 * kColWarps * bytes;
+      }
+    }
+    copies_commit();
+    fill = fill == (DEPTH - 1) * C::PAIR ? 0 : fill + C::PAIR;
+  };
+
+  Vec<16> token = read_token(first, 0);
+#pragma unroll 1
+  for (int i = 0; i < DEPTH - 1; ++i) fetch(first + col_warp + i * kColWarps);
+
+  float acc[MATS][4] = {};
+  int take = 0;  // offset of the slot to read next
+#pragma unroll 1
+  for (int slab = first; slab < last; slab += kSlab / 2) {
+    if (slab != first) {
+      __syncthreads();  // the digits have been read by all
+      token = read_token(slab, 0);
+    }
+#pragma unroll 1
+    for (int tok = 0;;) {
+      write_digits(token, tok);
+      if (++tok == tokens) break;
+      token = read_token(slab, tok);
+    }
+    __syncthreads();
+    const int end = last < slab + kSlab / 2 ? last : slab + kSlab / 2;
+#pragma unroll 1
+    for (int p = slab + col_warp; p < end; p += kColWarps) {
+      copies_wait<DEPTH - 2>();
+      __syncwarp();  // this pair is there for all lanes, and the one before has been read by all
+      fetch(p + (DEPTH - 1) * kColWarps);
+      if (!there) continue;
+      const float2 unit = *reinterpret_cast<const float2*>(units + (p - slab) * 8 + 2 * t);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (2 * p + h == s.col_tiles) break;
+        const int in_slab = 2 * (p - slab) + h;
+        // lanes whose column is past the last digit read the first one's; nobody reads their sums
+        const unsigned char* piece = digits + (in_slab * 2 * kDigitCols * 4 + (g < kDigitCols ? lane : t)) * 16;
+        const uint4 b0 = *reinterpret_cast<const uint4*>(piece);
+        const uint4 b1 = *reinterpret_cast<const uint4*>(piece + kDigitCols * 64);
+        const uint32_t b[4][2] = {{b0.x, b0.y}, {b0.z, b0.w}, {b1.x, b1.y}, {b1.z, b1.w}};
+#pragma unroll
+        for (int a = 0; a < MATS; ++a) {
+          const unsigned char* slot = ring + take + a * C::SLOT + h * block_bytes(GROUPS, w[a].zeros);
+          const uint4 lo4 = *reinterpret_cast<const uint4*>(slot + lane * 16);
+          const uint4 hi4 = *reinterpret_cast<const uint4*>(slot + 512 + lane * 16);
+          const uint32_t lo[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, hi[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
+          uint32_t d[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            constexpr int per_group = 4 / GROUPS;  // words per group
+            if (u % per_group == 0) d[0] = d[1] = d[2] = d[3] = kIntMagicBits;
+            imma(d, lo[u] & 0x0f0f0f0fu, hi[u] & 0x0f0f0f0fu, lo[u] >> 4 & 0x0f0f0f0fu, hi[u] >> 4 & 0x0f0f0f0fu,
+                 b[u][0], b[u][1]);
+            if ((u + 1) % per_group == 0) {
+              const int at = (g * GROUPS + u / per_group) * 2;
+              const uint32_t sc = *reinterpret_cast<const uint32_t*>(slot + kTileBytes + at * 2);
+              const float s_lo = H::to_float(sc & 0xffffu), s_hi = H::to_float(sc >> 16);
+              float z_lo = 8.0f, z_hi = 8.0f;
+              if (w[a].zeros) {
+                const uint32_t z = *reinterpret_cast<const uint16_t*>(slot + kTileBytes + GROUPS * 32 + at);
+                z_lo = zero_point(z & 0xffu);
+                z_hi = zero_point(z >> 8);
+              }
+              const float2 sum = *reinterpret_cast<const float2*>(digit_sums + (in_slab * GROUPS + u / per_group) * 8 + 2 * t);
+              // every term in front of the scale is an integer below 2^24: exact
+              acc[a][0] = fmaf(__uint_as_float(d[0]) + fmaf(-z_lo, sum.x, -kIntMagic), s_lo * unit.x, acc[a][0]);
+              acc[a][1] = fmaf(__uint_as_float(d[1]) + fmaf(-z_lo, sum.y, -kIntMagic), s_lo * unit.y, acc[a][1]);
+              acc[a][2] = fmaf(__uint_as_float(d[2]) + fmaf(-z_hi, sum.x, -kIntMagic), s_hi * unit.x, acc[a][2]);
+              acc[a][3] = fmaf(__uint_as_float(d[3]) + fmaf(-z_hi, sum.y, -kIntMagic), s_hi * unit.y, acc[a][3]);
+            }
+          }
+        }
+      }
+      take = take == (DEPTH - 1) * C::PAIR ? 0 : take + C::PAIR;
+    }
+  }
+
+  copies_wait<0>();
+  // A token's three columns, added up: token 0 is columns 0, 1, 2 and ends up in lanes t = 0, token 1 in lanes t = 1.
+  // Each rank finishes `slice` of the outputs [token][row]; what the warps have of it is stored there.
+  constexpr int kRows = kRowWarps * kTileRows;
+  const int outputs = tokens * kRows, slice = (outputs + split - 1) / split;
+  const uint32_t arrivals = smem_addr + C::RING + C::DIGITS + C::SUMS + C::UNITS;
+  cluster_wait();
+#pragma unroll
+  for (int a = 0; a < MATS; ++a)
+#pragma unroll
+    for (int hi = 0; hi < 2; ++hi) {
+      const float c0 = acc[a][2 * hi], c1 = acc[a][2 * hi + 1];
+      const float above = __shfl_down_sync(0xffffffffu, c0, 1), both = __shfl_down_sync(0xffffffffu, c0 + c1, 1);
+      const float v = t == 0 ? c0 + c1 + above : c1 + both;
+      const int o = t * kRows + row_warp * kTileRows + g + 8 * hi, owner = o / slice;
+      if (t < tokens)
+        cluster_store(arrivals + ((a * kColWarps + col_warp) * (kDigitOutputs + 64) + rank * slice + o - owner * slice) * 4,
+                      owner, v);
+    }
+  cluster_arrive();
+  cluster_wait();
+  const float* parts = reinterpret_cast<const float*>(smem + C::RING + C::DIGITS + C::SUMS + C::UNITS);
+  const int begin = rank * slice, o = threadIdx.x;  // slice <= kDigitOutputs <= 32 * kWarps
+  const int row = (begin + o) % kRows, tok = (begin + o) / kRows;
+  const long long n = (long long)row_tile0 * kTileRows + row;
+  if (o < slice && begin + o < outputs && n < s.n) {
+    float v[MATS];
+#pragma unroll
+    for (int a = 0; a < MATS; ++a) {
+      v[a] = 0.0f;
+#pragma unroll 1
+      for (int i = 0; i < split; ++i)
+#pragma unroll
+        for (int q = 0; q < kColWarps; ++q) v[a] += parts[(a * kColWarps + q) * (kDigitOutputs + 64) + i * slice + o];
+    }
+    const Consts consts(gm, dm);
+    static_cast<uint16_t*>(y)[(token0 + tok) * s.y_pitch + n] = H::from_float(result<MATS>(v, activation, consts));
   }
 }
 
@@ -212,13 +644,14 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(void* out, W4 w, W4S
   const long long row_tile = tile / s.col_tiles;
   const int c = (int)(tile - row_tile * s.col_tiles);
   if (row_tile * kTileRows >= s.n) return;
-  const char* p = cbyte(w.tiles) + tile * kTileBytes + lane * 16;
-  const Vec<16> q[2] = {Ld<16, LD_NC_NOALLOC>::ld(p), Ld<16, LD_NC_NOALLOC>::ld(p + 512)};
+  const int groups = 1 << s.groups_log2;
+  const char* block = cbyte(w.blocks) + tile * block_bytes(groups, w.zeros);
+  const Vec<16> q[2] = {Ld<16, LD_NC_NOALLOC>::ld(block + lane * 16), Ld<16, LD_NC_NOALLOC>::ld(block + 512 + lane * 16)};
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
-    const long long at = ((tile << s.groups_log2) + (u >> (2 - s.groups_log2))) * 16 + 2 * g;
-    const uint32_t sc = Ld<4, LD_PLAIN>::ld(cbyte(w.scales) + at * 2).w[0];
-    const uint32_t z = w.zeros ? Ld<2, LD_PLAIN>::ld(cbyte(w.zeros) + at).w[0] : 0x0808u;
+    const int at = (g * groups + (u >> (2 - s.groups_log2))) * 2;
+    const uint32_t sc = Ld<4, LD_PLAIN>::ld(block + kTileBytes + at * 2).w[0];
+    const uint32_t z = w.zeros ? Ld<2, LD_PLAIN>::ld(block + kTileBytes + groups * 32 + at).w[0] : 0x0808u;
 #pragma unroll
     for (int hi = 0; hi < 2; ++hi) {
       const long long row = row_tile * kTileRows + 8 * hi + g;
@@ -228,7 +661,7 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(void* out, W4 w, W4S
       const int zero = hi ? z >> 8 : z & 0xff;
       float f[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = (float)((int)(q[hi].w[u] >> (4 * e) & 15u) - zero) * scale;
+      for (int e = 0; e < 8; ++e) f[e] = (float)((int)(q[hi].w[u] >> (2 * e + 14 * (e & 1)) & 15u) - zero) * scale;
       Vec<16> v;
       Codec<T>::template pack<16>(f, v);
       char* dst = byte(out) + (row * s.y_pitch + k) * 2;
@@ -256,7 +689,7 @@ int launched() {
   return SWIGLU_B200_OK;
 }
 
-constexpr long long kMaxSize = 1LL << 40;  // of n and k: tile counts and byte offsets stay within 62 bits
+constexpr long long kMaxSize = 1LL << 31;  // of n and k: tile counts fit an int, byte offsets 62 bits
 
 // Checks shared by the three entries; fills the shape.
 int check(const W4* w, int mats, int64_t n, int64_t k, int group, int dtype, W4Shape& s) {
@@ -272,64 +705,140 @@ int check(const W4* w, int mats, int64_t n, int64_t k, int group, int dtype, W4S
   s.groups_log2 = group == 128 ? 0 : group == 64 ? 1 : 2;
   for (int i = 0; i < mats; ++i) {
     if (n == 0 || k == 0) break;
-    if (!w[i].tiles || !w[i].scales) return SWIGLU_B200_ERR_NULL;
-    if (address(w[i].tiles) % 16 || address(w[i].scales) % 4 || address(w[i].zeros) % 2) return SWIGLU_B200_ERR_ALIGN;
+    if (!w[i].blocks) return SWIGLU_B200_ERR_NULL;
+    if (address(w[i].blocks) % 16) return SWIGLU_B200_ERR_ALIGN;
   }
   return SWIGLU_B200_OK;
 }
 
-// Ranges that a call reads of one matrix.
-int weight_ranges(const W4& w, const W4Shape& s, ByteRange* r) {
+// The bytes that a call reads of one matrix.
+ByteRange weight_range(const W4& w, const W4Shape& s) {
   const long long tiles = (s.n + kTileRows - 1) / kTileRows * s.col_tiles;
-  const long long groups = (tiles << s.groups_log2) * kTileRows;
-  r[0] = byte_range(w.tiles, 1, tiles * kTileBytes, 0);
-  r[1] = byte_range(w.scales, 1, groups * 2, 0);
-  r[2] = w.zeros ? byte_range(w.zeros, 1, groups, 0) : ByteRange{0, 0};
-  return 3;
+  return byte_range(w.blocks, 1, tiles * block_bytes(1 << s.groups_log2, w.zeros), 0);
 }
 
-template <class T, int MATS, int NT, int ACT>
-int launch(void* y, const void* x, const W4* w, const W4Shape& s, float gm, float dm, cudaStream_t st) {
-  // Two weight tiles to a warp where a token tile of 32 is read beside them: its fragments are 8 KB per column tile, 8
-  // times the weights of one tile.
+// SMs of the current device, asked for once.
+int sm_count(int& sms) {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return note_cuda_error(SWIGLU_B200_ERR_DEVICE, e);
+  sms = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (sms == 0) {
+    e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return note_cuda_error(SWIGLU_B200_ERR_DEVICE, e);
+    if (dev < 64) known[dev].store(sms, std::memory_order_relaxed);
+  }
+  return SWIGLU_B200_OK;
+}
+
+// Launches `kernel` in clusters of `split` CTAs along x, raising its limit of shared memory on its first use on a device
+// (`opted_in`: one bit per device).
+template <class... P, class... A>
+int start(void (*kernel)(P...), std::atomic<uint64_t>& opted_in, dim3 grid, int split, int smem, cudaStream_t st,
+          A... args) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && !(dev < 64 && (opted_in.load(std::memory_order_relaxed) >> dev & 1))) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess && dev < 64) opted_in.fetch_or(1ULL << dev, std::memory_order_relaxed);
+  }
+  if (e != cudaSuccess) return note_cuda_error(SWIGLU_B200_ERR_DEVICE, e);
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = (unsigned)split;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(32 * kWarps);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cfg.attrs = &cluster;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return note_cuda_error(SWIGLU_B200_ERR_LAUNCH, e);
+  }
+  note_launch();
+  return SWIGLU_B200_OK;
+}
+
+// Parts that the column tiles (or pairs) are cut into: as many CTAs as run at once, so that all of them stream from the
+// start and end together.
+int split_of(long long ctas, int parts, long long slots) {
+  long long split = slots / ctas;
+  if (split > parts) split = parts;
+  return split < 1 ? 1 : split > 8 ? 8 : (int)split;
+}
+
+template <class T, int MATS, int NT, int GROUPS>
+int launch(void* y, const void* x, const W4* w, W4Shape s, int activation, float gm, float dm,
+           cudaStream_t st) {
+  // Two weight tiles to a warp where 32 tokens are read beside them: the fragments of those are 8 KB per column tile,
+  // 8 times the codes of one tile.
   constexpr int RT = NT == 4 && MATS == 1 ? 2 : 1;
+  using C = Cfg<MATS, RT, NT, GROUPS>;
+  static std::atomic<uint64_t> opted_in{0};
   const long long row_tiles = (s.n + kTileRows - 1) / kTileRows;
-  const long long gx = (row_tiles + RT - 1) / RT, gy = (s.m + 8 * NT - 1) / (8 * NT);
-  if (gx > 0x7fffffffLL || gy > 65535) return SWIGLU_B200_ERR_SHAPE;
-  w4_kernel<T, MATS, RT, NT, ACT><<<dim3((unsigned)gx, (unsigned)gy), 32 * kWarps, 0, st>>>(
-      y, x, w[0], MATS == 2 ? w[1] : w[0], s, gm, dm);
-  return launched();
+  const long long row_ctas = (row_tiles + kWarps * RT - 1) / (kWarps * RT), gy = (s.m + 8 * NT - 1) / (8 * NT);
+  if (row_ctas > 0x7fffffffLL / 8 || gy > 65535) return SWIGLU_B200_ERR_SHAPE;
+  int sms = 0;
+  const int rc = sm_count(sms);
+  if (rc != SWIGLU_B200_OK) return rc;
+  s.split = split_of(row_ctas * gy, s.col_tiles, (long long)sms * C::CTAS);
+  return start(w4_kernel<T, MATS, RT, NT, GROUPS>, opted_in, dim3((unsigned)(row_ctas * s.split), (unsigned)gy),
+               s.split, C::SMEM, st, y, x, w[0], w[MATS - 1], s, activation, gm, dm);
 }
 
-template <int MATS, int ACT>
+template <class T, int MATS, int GROUPS>
+int launch_digits(void* y, const void* x, const W4* w, W4Shape s, int activation, float gm, float dm,
+                  cudaStream_t st) {
+  using C = DigitCfg<MATS, GROUPS>;
+  static std::atomic<uint64_t> opted_in{0};
+  const long long row_tiles = (s.n + kTileRows - 1) / kTileRows, row_ctas = (row_tiles + kRowWarps - 1) / kRowWarps;
+  const long long gy = (s.m + kDigitTokens - 1) / kDigitTokens;
+  if (row_ctas > 0x7fffffffLL / 8 || gy > 65535) return SWIGLU_B200_ERR_SHAPE;
+  int sms = 0;
+  const int rc = sm_count(sms);
+  if (rc != SWIGLU_B200_OK) return rc;
+  s.split = split_of(row_ctas * gy, (s.col_tiles + 1) / 2, 3LL * sms);
+  return start(w4_digits_kernel<T, MATS, GROUPS>, opted_in, dim3((unsigned)(row_ctas * s.split), (unsigned)gy),
+               s.split, C::SMEM, st, y, x, w[0], w[MATS - 1], s, activation, gm, dm);
+}
+
+template <int MATS>
 int run(void* y, const void* x, const W4* w, W4Shape s, int64_t m, int64_t x_row_stride, int64_t y_row_stride,
-        int dtype, float gm, float dm, int device, void* stream) {
+        int dtype, int activation, float gm, float dm, int device, void* stream) {
   if (m < 0) return SWIGLU_B200_ERR_SHAPE;
   if (m == 0 || s.n == 0) return SWIGLU_B200_OK;
   if (s.k == 0) return SWIGLU_B200_ERR_SHAPE;
   if (x_row_stride < s.k || y_row_stride < s.n) return SWIGLU_B200_ERR_SHAPE;
   if (!fits_address_space(m, x_row_stride, 2) || !fits_address_space(m, y_row_stride, 2)) return SWIGLU_B200_ERR_SHAPE;
   if (!y || !x) return SWIGLU_B200_ERR_NULL;
-  if (address(y) % 2 || address(x) % 2) return SWIGLU_B200_ERR_ALIGN;
+  if (address(y) % 2 || address(x) % 16 || (m > 1 && x_row_stride % 8)) return SWIGLU_B200_ERR_ALIGN;
   const ByteRange out = byte_range(y, m, s.n * 2, y_row_stride * 2);
-  ByteRange in[7];
-  in[0] = byte_range(x, m, s.k * 2, x_row_stride * 2);
-  int count = 1;
-  for (int i = 0; i < MATS; ++i) count += weight_ranges(w[i], s, in + count);
-  for (int i = 0; i < count; ++i)
-    if (overlap(out, in[i])) return SWIGLU_B200_ERR_ALIAS;
+  if (overlap(out, byte_range(x, m, s.k * 2, x_row_stride * 2))) return SWIGLU_B200_ERR_ALIAS;
+  for (int i = 0; i < MATS; ++i)
+    if (overlap(out, weight_range(w[i], s))) return SWIGLU_B200_ERR_ALIAS;
   CallDevice scope(device);
   if (scope.err != cudaSuccess) return note_cuda_error(SWIGLU_B200_ERR_DEVICE, scope.err);
   s.m = m;
   s.x_pitch = x_row_stride;
   s.y_pitch = y_row_stride;
-  s.x_vec = address(x) % 16 == 0 && (m == 1 || x_row_stride % 8 == 0);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto typed = [&](auto t) {
     using T = decltype(t);
-    if (m <= 8) return launch<T, MATS, 1, ACT>(y, x, w, s, gm, dm, st);
-    if (m <= 16) return launch<T, MATS, 2, ACT>(y, x, w, s, gm, dm, st);
-    return launch<T, MATS, 4, ACT>(y, x, w, s, gm, dm, st);
+    auto grouped = [&](auto groups) {
+      constexpr int G = decltype(groups)::value;
+      if (m <= kDigitTokens) return launch_digits<T, MATS, G>(y, x, w, s, activation, gm, dm, st);
+      if (m <= 8) return launch<T, MATS, 1, G>(y, x, w, s, activation, gm, dm, st);
+      if (m <= 16) return launch<T, MATS, 2, G>(y, x, w, s, activation, gm, dm, st);
+      return launch<T, MATS, 4, G>(y, x, w, s, activation, gm, dm, st);
+    };
+    if (s.groups_log2 == 0) return grouped(std::integral_constant<int, 1>{});
+    if (s.groups_log2 == 1) return grouped(std::integral_constant<int, 2>{});
+    return grouped(std::integral_constant<int, 4>{});
   };
   return dtype == SWIGLU_B200_F16 ? typed(__half{}) : typed(__nv_bfloat16{});
 }
@@ -338,38 +847,29 @@ int run(void* y, const void* x, const W4* w, W4Shape s, int64_t m, int64_t x_row
 
 extern "C" {
 
-int swiglu_b200_w4_linear(void* y, const void* x, const void* tiles, const void* scales, const void* zeros, int64_t m,
-                          int64_t n, int64_t k, int64_t x_row_stride, int64_t y_row_stride, int group, int dtype,
-                          int device, void* stream) {
-  const W4 w{tiles, scales, zeros};
+int swiglu_b200_w4_linear(void* y, const void* x, const void* blocks, int zeros, int64_t m, int64_t n, int64_t k,
+                          int64_t x_row_stride, int64_t y_row_stride, int group, int dtype, int device, void* stream) {
+  const W4 w{blocks, zeros != 0};
   W4Shape s{};
   const int rc = check(&w, 1, n, k, group, dtype, s);
   if (rc != SWIGLU_B200_OK) return rc;
-  return run<1, ACT_SILU>(y, x, &w, s, m, x_row_stride, y_row_stride, dtype, 1.0f, 1.0f, device, stream);
+  return run<1>(y, x, &w, s, m, x_row_stride, y_row_stride, dtype, SWIGLU_B200_SILU, 1.0f, 1.0f, device, stream);
 }
 
-int swiglu_b200_w4_gate_up(void* h, const void* x, const void* gate_tiles, const void* gate_scales,
-                           const void* gate_zeros, const void* up_tiles, const void* up_scales, const void* up_zeros,
-                           int64_t m, int64_t n, int64_t k, int64_t x_row_stride, int64_t h_row_stride, int group,
-                           int dtype, int activation, float gm, float dm, int device, void* stream) {
-  const W4 w[2] = {{gate_tiles, gate_scales, gate_zeros}, {up_tiles, up_scales, up_zeros}};
+int swiglu_b200_w4_gate_up(void* h, const void* x, const void* gate_blocks, int gate_zeros, const void* up_blocks,
+                           int up_zeros, int64_t m, int64_t n, int64_t k, int64_t x_row_stride, int64_t h_row_stride,
+                           int group, int dtype, int activation, float gm, float dm, int device, void* stream) {
+  const W4 w[2] = {{gate_blocks, gate_zeros != 0}, {up_blocks, up_zeros != 0}};
   W4Shape s{};
   const int rc = check(w, 2, n, k, group, dtype, s);
   if (rc != SWIGLU_B200_OK) return rc;
-  switch (activation) {
-    case SWIGLU_B200_SILU:
-      return run<2, ACT_SILU>(h, x, w, s, m, x_row_stride, h_row_stride, dtype, gm, dm, device, stream);
-    case SWIGLU_B200_GELU_TANH:
-      return run<2, ACT_GELU_TANH>(h, x, w, s, m, x_row_stride, h_row_stride, dtype, gm, dm, device, stream);
-    case SWIGLU_B200_GELU_ERF:
-      return run<2, ACT_GELU_ERF>(h, x, w, s, m, x_row_stride, h_row_stride, dtype, gm, dm, device, stream);
-    default: return SWIGLU_B200_ERR_ARG;
-  }
+  if (activation < SWIGLU_B200_SILU || activation > SWIGLU_B200_GELU_ERF) return SWIGLU_B200_ERR_ARG;
+  return run<2>(h, x, w, s, m, x_row_stride, h_row_stride, dtype, activation, gm, dm, device, stream);
 }
 
-int swiglu_b200_w4_dequantize(void* out, const void* tiles, const void* scales, const void* zeros, int64_t n,
-                              int64_t k, int64_t out_row_stride, int group, int dtype, int device, void* stream) {
-  const W4 w{tiles, scales, zeros};
+int swiglu_b200_w4_dequantize(void* out, const void* blocks, int zeros, int64_t n, int64_t k, int64_t out_row_stride,
+                              int group, int dtype, int device, void* stream) {
+  const W4 w{blocks, zeros != 0};
   W4Shape s{};
   const int rc = check(&w, 1, n, k, group, dtype, s);
   if (rc != SWIGLU_B200_OK) return rc;
@@ -378,10 +878,7 @@ int swiglu_b200_w4_dequantize(void* out, const void* tiles, const void* scales, 
   if (!out) return SWIGLU_B200_ERR_NULL;
   if (address(out) % 2) return SWIGLU_B200_ERR_ALIGN;
   const ByteRange o = byte_range(out, n, k * 2, out_row_stride * 2);
-  ByteRange in[3];
-  weight_ranges(w, s, in);
-  for (const ByteRange& r : in)
-    if (overlap(o, r)) return SWIGLU_B200_ERR_ALIAS;
+  if (overlap(o, weight_range(w, s))) return SWIGLU_B200_ERR_ALIAS;
   const long long tiles_all = (n + kTileRows - 1) / kTileRows * s.col_tiles, ctas = (tiles_all + 7) / 8;
   if (ctas > 0x7fffffffLL) return SWIGLU_B200_ERR_SHAPE;
   CallDevice scope(device);

@@ -30,12 +30,23 @@ from .swiglu import _DTYPE_CODE, _stream
 
 DTYPES = (torch.bfloat16, torch.float16)
 GROUP_SIZES = (32, 64, 128)
-TILE_ROWS, TILE_COLS = 16, 128
+TILE_ROWS, TILE_COLS, CODE_BYTES = 16, 128, 1024
 MATVEC_ROWS = 32
 
 
 def _ceil(a: int, b: int) -> int:
     return (a + b - 1) // b
+
+
+# Nibbles of a 32-bit word: the plain order is by column, in a block columns (0, 2, 4, 6, 1, 3, 5, 7).
+_TO_BLOCK = (0, 2, 4, 6, 1, 3, 5, 7)
+_FROM_BLOCK = (0, 4, 1, 5, 2, 6, 3, 7)
+
+
+def _shuffle(p: torch.Tensor, order) -> torch.Tensor:
+    """Bytes in words of four along the last dimension, with nibble ``order[i]`` of each word moved to place i."""
+    q = torch.stack((p & 15, p >> 4), dim=-1).flatten(-2)[..., list(order)]
+    return q[..., 0::2] | (q[..., 1::2] << 4)
 
 
 class W4Weight:
@@ -45,10 +56,10 @@ class W4Weight:
     ``scales``  bf16 or fp16 ``[n, ceil(k / group_size)]``, the dtype of the tokens it multiplies;
     ``zeros``   uint8 of the shape of ``scales``, 0..15, or ``None`` for 8 everywhere.
 
-    The constructor lays them out once in the tiles the kernels read (``swiglu_b200_w4_linear`` in the C header) and
-    keeps only those; ``packed``, ``scales`` and ``zeros`` are rebuilt on request."""
+    The constructor lays them out once in ``blocks``, the form the kernels read (``swiglu_b200_w4_linear`` in the C
+    header), and keeps only that; ``packed``, ``scales`` and ``zeros`` are rebuilt on request."""
 
-    __slots__ = ("tiles", "tile_scales", "tile_zeros", "out_features", "in_features", "group_size", "_pointers")
+    __slots__ = ("blocks", "dtype", "out_features", "in_features", "group_size", "has_zeros", "_operand")
 
     def __init__(self, packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, *,
                  in_features: int, group_size: int = 128):
@@ -74,85 +85,87 @@ class W4Weight:
                 raise ValueError("zeros must lie in 0..15")
         if any(t is not None and t.device != packed.device for t in (scales, zeros)):
             raise ValueError("packed, scales and zeros must be on one device")
-        self.out_features, self.in_features, self.group_size = n, k, group_size
-        rows, cols = _ceil(n, TILE_ROWS), _ceil(k, TILE_COLS)
+        self.dtype, self.out_features, self.in_features, self.group_size = scales.dtype, n, k, group_size
+        self.has_zeros = zeros is not None
+        rows, cols = self._tiles()
         # [row tile, 2, 8, column tile, word u, lane t, byte] -> [row tile, column tile, 2, 8, t, u, byte]
         p = torch.nn.functional.pad(packed, (0, 64 * cols - packed.shape[1], 0, TILE_ROWS * rows - n))
-        self.tiles = p.reshape(rows, 2, 8, cols, 4, 4, 4).permute(0, 3, 1, 2, 5, 4, 6).contiguous()
-        self.tile_scales = self._tile_groups(scales)
-        self.tile_zeros = None if zeros is None else self._tile_groups(zeros)
-        self._set_pointers()
+        p = _shuffle(p.reshape(rows, 2, 8, cols, 4, 4, 4), _TO_BLOCK)
+        parts = [p.permute(0, 3, 1, 2, 5, 4, 6).reshape(rows, cols, -1), self._tile_groups(scales)]
+        if zeros is not None:
+            parts.append(self._tile_groups(zeros))
+        self._set_blocks(torch.cat(parts, dim=2))
 
-    def _set_pointers(self) -> None:
-        self._pointers = (self.tiles.data_ptr(), self.tile_scales.data_ptr(),
-                          None if self.tile_zeros is None else self.tile_zeros.data_ptr())
+    def _set_blocks(self, blocks: torch.Tensor) -> None:
+        self.blocks = blocks  # uint8 [row tiles, column tiles, bytes of a block]
+        self._operand = (blocks.data_ptr(), int(self.has_zeros))
 
-    def _groups(self) -> int:
-        return _ceil(self.in_features, TILE_COLS) * (TILE_COLS // self.group_size)
+    def _tiles(self):
+        return _ceil(self.out_features, TILE_ROWS), _ceil(self.in_features, TILE_COLS)
 
     def _tile_groups(self, t: torch.Tensor) -> torch.Tensor:
-        """[n, groups] -> [row tile, group, 8, 2], zero past the matrix."""
-        rows, groups = self.tiles.shape[0], self._groups()
-        t = torch.nn.functional.pad(t, (0, groups - t.shape[1], 0, TILE_ROWS * rows - t.shape[0]))
-        return t.reshape(rows, 2, 8, groups).permute(0, 3, 2, 1).contiguous()
+        """[n, groups] -> bytes [row tile, column tile, (8, group, 2)], zero past the matrix."""
+        (rows, cols), per = self._tiles(), TILE_COLS // self.group_size
+        t = torch.nn.functional.pad(t, (0, cols * per - t.shape[1], 0, TILE_ROWS * rows - t.shape[0]))
+        t = t.reshape(rows, 2, 8, cols, per).permute(0, 3, 2, 4, 1).reshape(rows, cols, -1)
+        return t.contiguous().view(torch.uint8)
 
-    def _untile_groups(self, t: torch.Tensor) -> torch.Tensor:
-        rows = t.permute(0, 3, 2, 1).reshape(-1, self._groups())
-        return rows[:self.out_features, :_ceil(self.in_features, self.group_size)].contiguous()
+    def _untile_groups(self, lo: int, dtype: torch.dtype) -> torch.Tensor:
+        (rows, cols), per = self._tiles(), TILE_COLS // self.group_size
+        t = self.blocks[:, :, lo:lo + 16 * per * dtype.itemsize].contiguous().view(dtype)
+        t = t.view(rows, cols, 8, per, 2).permute(0, 4, 2, 1, 3).reshape(TILE_ROWS * rows, cols * per)
+        return t[:self.out_features, :_ceil(self.in_features, self.group_size)].contiguous()
 
     @property
     def packed(self) -> torch.Tensor:
-        rows, cols = self.tiles.shape[:2]
-        p = self.tiles.permute(0, 2, 3, 1, 5, 4, 6).reshape(TILE_ROWS * rows, 64 * cols)
+        rows, cols = self._tiles()
+        p = self.blocks[:, :, :CODE_BYTES].reshape(rows, cols, 2, 8, 4, 4, 4).permute(0, 2, 3, 1, 5, 4, 6)
+        p = _shuffle(p, _FROM_BLOCK).reshape(TILE_ROWS * rows, 64 * cols)
         return p[:self.out_features, :16 * _ceil(self.in_features, 32)].contiguous()
 
     @property
     def scales(self) -> torch.Tensor:
-        return self._untile_groups(self.tile_scales)
+        return self._untile_groups(CODE_BYTES, self.dtype)
 
     @property
     def zeros(self) -> Optional[torch.Tensor]:
-        return None if self.tile_zeros is None else self._untile_groups(self.tile_zeros)
+        if not self.has_zeros:
+            return None
+        return self._untile_groups(CODE_BYTES + 32 * (TILE_COLS // self.group_size), torch.uint8)
 
     @property
     def shape(self) -> torch.Size:
         return torch.Size((self.out_features, self.in_features))
 
     @property
-    def dtype(self) -> torch.dtype:
-        return self.tile_scales.dtype
-
-    @property
     def device(self) -> torch.device:
-        return self.tiles.device
+        return self.blocks.device
 
     @property
     def nbytes(self) -> int:
         """Bytes the kernels read of it."""
-        parts = (self.tiles, self.tile_scales, self.tile_zeros)
-        return sum(t.numel() * t.element_size() for t in parts if t is not None)
+        return self.blocks.numel()
 
     def to(self, device) -> "W4Weight":
         """This weight on ``device`` (itself when it is there already)."""
-        moved = self.tiles.to(device)
-        if moved is self.tiles:
+        moved = self.blocks.to(device)
+        if moved is self.blocks:
             return self
         other = object.__new__(W4Weight)
-        other.out_features, other.in_features, other.group_size = self.out_features, self.in_features, self.group_size
-        other.tiles, other.tile_scales = moved, self.tile_scales.to(device)
-        other.tile_zeros = None if self.tile_zeros is None else self.tile_zeros.to(device)
-        other._set_pointers()
+        for name in ("dtype", "out_features", "in_features", "group_size", "has_zeros"):
+            setattr(other, name, getattr(self, name))
+        other._set_blocks(moved)
         return other
 
     def dequantize(self) -> torch.Tensor:
         """``[out_features, in_features]`` in the dtype of the scales: ``(code - zero) * scale`` rounded once."""
-        if not self.tiles.is_cuda:
+        if not self.blocks.is_cuda:
             raise RuntimeError("W4Weight.dequantize has a CUDA (sm_100a) kernel only; there is no CPU fallback")
         n, k = self.shape
         out = torch.empty((n, k), dtype=self.dtype, device=self.device)
         _lib.check(
             "W4Weight.dequantize",
-            _lib.lib.swiglu_b200_w4_dequantize(out.data_ptr(), *self._pointers, n, k, k, self.group_size,
+            _lib.lib.swiglu_b200_w4_dequantize(out.data_ptr(), *self._operand, n, k, k, self.group_size,
                                                _DTYPE_CODE[self.dtype], self.device.index, _stream(self.device)),
         )
         return out
@@ -203,7 +216,7 @@ def quantize_w4(weight: torch.Tensor, group_size: int = 128, zero_points: bool =
 
 
 def _check_tokens(x: torch.Tensor, w: W4Weight, what: str) -> None:
-    if not (x.is_cuda and w.tiles.is_cuda):
+    if not (x.is_cuda and w.blocks.is_cuda):
         raise RuntimeError(f"{what} has a CUDA (sm_100a) kernel only; there is no CPU fallback")
     if x.device != w.device:
         raise ValueError(f"x is on {x.device}, the weight on {w.device}")
@@ -215,6 +228,19 @@ def _check_tokens(x: torch.Tensor, w: W4Weight, what: str) -> None:
         raise RuntimeError(f"{what} is forward only (frozen 4-bit weights): call it under torch.no_grad()")
 
 
+def _aligned_rows(x: torch.Tensor):
+    """The rows of ``x`` where every row starts on a 16-byte boundary, as the kernels need them, and their pitch; copied
+    into padded rows when they do not."""
+    rows, pitch = _rows(x)
+    if rows.data_ptr() % 16 == 0 and (pitch % 8 == 0 or x.shape[:-1].numel() == 1):
+        return rows, pitch
+    k = x.shape[-1]
+    pitch = 8 * _ceil(k, 8)
+    rows = x.new_empty((*x.shape[:-1], pitch))
+    rows[..., :k] = x
+    return rows, pitch
+
+
 def w4_linear(x: torch.Tensor, weight: W4Weight) -> torch.Tensor:
     """``x W^T`` for ``x`` ``[..., in_features]`` of the weight's dtype."""
     _check_tokens(x, weight, "w4_linear")
@@ -223,11 +249,11 @@ def w4_linear(x: torch.Tensor, weight: W4Weight) -> torch.Tensor:
     if m > MATVEC_ROWS:
         return x @ weight.dequantize().t()
     y = x.new_empty((*x.shape[:-1], n))
-    x, pitch = _rows(x)
+    x, pitch = _aligned_rows(x)
     device = x.device
     _lib.check(
         "w4_linear",
-        _lib.lib.swiglu_b200_w4_linear(y.data_ptr(), x.data_ptr(), *weight._pointers, m, n, k, pitch, n,
+        _lib.lib.swiglu_b200_w4_linear(y.data_ptr(), x.data_ptr(), *weight._operand, m, n, k, pitch, n,
                                        weight.group_size, _DTYPE_CODE[x.dtype], device.index, _stream(device)),
     )
     return y
@@ -266,12 +292,12 @@ def w4_gate_up(x: torch.Tensor, w_gate: W4Weight, w_up: W4Weight, activation: st
     if m > MATVEC_ROWS:
         return _gate_up_16bit(x, w_gate, w_up, activation, gm, dm)
     h = x.new_empty((*x.shape[:-1], n))
-    x, pitch = _rows(x)
+    x, pitch = _aligned_rows(x)
     device = x.device
     _lib.check(
         "w4_gate_up",
         _lib.lib.swiglu_b200_w4_gate_up(
-            h.data_ptr(), x.data_ptr(), *w_gate._pointers, *w_up._pointers, m, n, k, pitch, n, w_gate.group_size,
+            h.data_ptr(), x.data_ptr(), *w_gate._operand, *w_up._operand, m, n, k, pitch, n, w_gate.group_size,
             _DTYPE_CODE[x.dtype], ACTIVATIONS[activation], gm, dm, device.index, _stream(device),
         ),
     )

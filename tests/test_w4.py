@@ -93,14 +93,21 @@ def test_layout_goes_there_and_back(n, k, group, zeros):
     assert torch.equal(w.packed, packed) and torch.equal(w.scales, scales)
     assert w.zeros is None if z is None else torch.equal(w.zeros, z)
     assert w.shape == (n, k) and w.dtype == torch.bfloat16 and w.to("cpu") is w
-    # the documented place of one code: tile (r, c), word (hi, g, t, u), nibble i
-    words = w.tiles.contiguous().view(-1).view(torch.int32).view(*w.tiles.shape[:-1])
+    # the documented place of one code: block (r, c), word (hi, g, t, u), its half by parity; and of its scale
+    rows, cols, per = (n + 15) // 16, (k + 127) // 128, 128 // group
+    size = 1024 + 32 * per + (16 * per if zeros else 0)
+    assert w.blocks.shape == (rows, cols, size) and w.nbytes == rows * cols * size
+    words = w.blocks[:, :, :1024].contiguous().view(torch.int32).view(rows, cols, 2, 8, 4, 4)
+    tail = w.blocks[:, :, 1024:]
     for row, col in ((0, 0), (n - 1, k - 1), (n // 2, k // 2)):
-        r, c, i = row // 16, col // 128, col % 8
+        r, c, i = row // 16, col // 128, col % 8 // 2 + col % 2 * 4
         word = int(words[r, c, row // 8 % 2, row % 8, col // 8 % 4, col // 32 % 4]) & 0xffffffff
         byte = int(packed[row, col // 2])
         assert word >> (4 * i) & 15 == (byte >> 4 if col & 1 else byte & 15)
-    assert w.nbytes == w.tiles.numel() + 2 * w.tile_scales.numel() + (w.tile_zeros.numel() if zeros else 0)
+        at = (row % 8 * per + col % 128 // group) * 2 + row // 8 % 2
+        assert tail[r, c, 2 * at:2 * at + 2].contiguous().view(torch.bfloat16) == scales[row, col // group]
+        if zeros:
+            assert tail[r, c, 32 * per + at] == z[row, col // group]
 
 
 @pytest.mark.parametrize("zero_points", [False, True])
@@ -170,35 +177,36 @@ def test_refusals():
 def test_c_entries_refuse_bad_arguments_without_a_device():
     lin, gu, dq = _lib.lib.swiglu_b200_w4_linear, _lib.lib.swiglu_b200_w4_gate_up, _lib.lib.swiglu_b200_w4_dequantize
     p = 0x100000
-    y, x, t, s, z = (p + i * 0x10000 for i in range(5))
+    y, x, w = (p + i * 0x10000 for i in range(3))
 
-    def linear(y=y, x=x, t=t, s=s, z=z, m=2, n=20, k=130, sx=130, sy=20, group=64, dtype=1):
-        return lin(y, x, t, s, z, m, n, k, sx, sy, group, dtype, -1, None)
+    def linear(y=y, x=x, w=w, m=2, n=20, k=130, sx=136, sy=20, group=64, dtype=1):
+        return lin(y, x, w, 1, m, n, k, sx, sy, group, dtype, -1, None)
 
     assert linear(dtype=0) == 1 and linear(dtype=5) == 1
     assert linear(group=16) == 10 and linear(group=0) == 10
-    for bad in (dict(m=-1), dict(n=-1), dict(k=-1), dict(sx=129), dict(sy=19), dict(k=0), dict(n=1 << 50, k=1 << 50),
+    for bad in (dict(m=-1), dict(n=-1), dict(k=-1), dict(sx=129), dict(sy=19), dict(k=0), dict(n=1 << 32), dict(k=1 << 32),
                 dict(m=1 << 40, sx=1 << 40)):
         assert linear(**bad) == 3
-    for name in ("y", "x", "t", "s"):
+    for name in ("y", "x", "w"):
         assert linear(**{name: None}) == 2
-    assert linear(x=x + 1) == 4 and linear(y=y + 1) == 4 and linear(t=t + 8) == 4 and linear(s=s + 2) == 4
-    assert linear(z=z + 1) == 4
-    assert linear(y=x + 8) == 5 and linear(y=t + 512) == 5 and linear(y=s) == 5 and linear(y=z) == 5
+    assert linear(x=x + 2) == 4 and linear(sx=130) == 4 and linear(y=y + 1) == 4 and linear(w=w + 8) == 4
+    assert linear(y=x + 8) == 5 and linear(y=w + 512) == 5
+    # two row tiles of two blocks of 1024 codes, two scales and two zero points for each of 16 rows
+    assert linear(y=w + 4 * (1024 + 64 + 32) - 2) == 5
     assert linear(m=0, y=None, x=None) == 0 and linear(n=0, sy=0) == 0
 
-    def gate_up(h=y, act=0, ut=p + 0x60000, dtype=2, dm=1.0):
-        return gu(h, x, t, s, z, ut, p + 0x70000, None, 2, 20, 130, 130, 20, 32, dtype, act, 1.0, dm, -1, None)
+    def gate_up(h=y, act=0, u=p + 0x60000, dtype=2):
+        return gu(h, x, w, 1, u, 0, 2, 20, 130, 136, 20, 32, dtype, act, 1.0, 1.0, -1, None)
 
-    assert gate_up(act=3) == 10 and gate_up(act=-1) == 10 and gate_up(dtype=0) == 1 and gate_up(ut=None) == 2
-    assert gate_up(h=p + 0x60000) == 5 and gate_up(h=p + 0x70000) == 5
+    assert gate_up(act=3) == 10 and gate_up(act=-1) == 10 and gate_up(dtype=0) == 1 and gate_up(u=None) == 2
+    assert gate_up(h=p + 0x60000) == 5 and gate_up(h=w + 2) == 5
 
-    def dequantize(out=y, n=20, k=130, so=130, group=128, dtype=1, t=t):
-        return dq(out, t, s, z, n, k, so, group, dtype, -1, None)
+    def dequantize(out=y, n=20, k=130, so=130, group=128, dtype=1, w=w):
+        return dq(out, w, 1, n, k, so, group, dtype, -1, None)
 
     assert dequantize(dtype=0) == 1 and dequantize(group=256) == 10 and dequantize(so=129) == 3
-    assert dequantize(out=None) == 2 and dequantize(t=None) == 2 and dequantize(out=y + 1) == 4
-    assert dequantize(out=t) == 5 and dequantize(n=0, out=None) == 0 and dequantize(k=0, so=0) == 0
+    assert dequantize(out=None) == 2 and dequantize(w=None) == 2 and dequantize(out=y + 1) == 4
+    assert dequantize(out=w) == 5 and dequantize(n=0, out=None) == 0 and dequantize(k=0, so=0) == 0
 
 
 # ------------------------------------------------------------------------------------ values
@@ -275,14 +283,14 @@ def test_pitched_and_misaligned_tokens(dtype, m, offset, extra):
     out = torch.full((16 + m * (n + 5),), 55.0, dtype=dtype, device="cuda")
     y = out[8:8 + m * (n + 5)].view(m, n + 5)[:, :n]
     st = torch.cuda.current_stream().cuda_stream
-    assert _lib.lib.swiglu_b200_w4_linear(y.data_ptr(), x.data_ptr(), *w._pointers, m, n, k, k, n + 5, 64,
+    assert _lib.lib.swiglu_b200_w4_linear(y.data_ptr(), x.data_ptr(), *w._operand, m, n, k, k, n + 5, 64,
                                           CODES[dtype], -1, st) == 0
     assert torch.equal(y, want)
     y.fill_(55.0)
     assert bool((out == 55.0).all())
     full = torch.full((n * (k + 7) + 16,), 55.0, dtype=dtype, device="cuda")
     d = full[5:5 + n * (k + 7)].view(n, k + 7)[:, :k]
-    assert _lib.lib.swiglu_b200_w4_dequantize(d.data_ptr(), *w._pointers, n, k, k + 7, 64, CODES[dtype], -1, st) == 0
+    assert _lib.lib.swiglu_b200_w4_dequantize(d.data_ptr(), *w._operand, n, k, k + 7, 64, CODES[dtype], -1, st) == 0
     assert torch.equal(d, w.dequantize())
     d.fill_(55.0)
     assert bool((full == 55.0).all())
