@@ -216,9 +216,14 @@ __device__ __forceinline__ uint32_t step_load(const void* steps, const Ckpt8Shap
 
 constexpr int kWarps = 4;  // most warps of a CTA
 
+// CTAs to an SM that the registers are budgeted for (bf16 [16384, 14336], 6 / 8 / 10 / 16 of them: forward 283 / 276 / 277 /
+// 304 us; backward with 6 / 8 / 10 / 12: 385 / 301 / 289 / 292 us, at half-width 11009 packed 103 / 90 / 77 / 78 us; with h
+// 385 / 359 / 357 / 445 us, where GELU loses 3 % from 8 to 10 and the skewed form gains 4 %).
+constexpr int kForwardCtas = 10, kBackwardCtas = 10, kBackwardHCtas = 8;
+
 // h may be NULL: the codes alone are stored.
 template <class T, int ACT, bool SKEW>
-__global__ void __launch_bounds__(32 * kWarps, 8)
+__global__ void __launch_bounds__(32 * kWarps, kForwardCtas)
 ckpt8_fwd_kernel(void* h, void* gate_codes, void* up_codes, void* gate_steps, void* up_steps,
                  const void* __restrict__ gate, const void* __restrict__ up, Ckpt8Shape s, float gm, float dm) {
   constexpr bool FAST = (sizeof(T) == 2);
@@ -251,7 +256,7 @@ ckpt8_fwd_kernel(void* h, void* gate_codes, void* up_codes, void* gate_steps, vo
 // With H, h = act(gate*gm) * up * dm of the kept values is stored too; it may overwrite dout (a warp stores only
 // elements whose values its own lanes have read by then).
 template <class T, int ACT, bool SKEW, bool H>
-__global__ void __launch_bounds__(32 * kWarps, 8)
+__global__ void __launch_bounds__(32 * kWarps, H && !SKEW ? kBackwardHCtas : kBackwardCtas)
 ckpt8_bwd_kernel(void* h, void* dgate, void* dup, const void* dout, const void* __restrict__ gate_codes,
                  const void* __restrict__ up_codes, const void* __restrict__ gate_steps,
                  const void* __restrict__ up_steps, Ckpt8Shape s, float gm, float dm) {
