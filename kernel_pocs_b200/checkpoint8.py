@@ -96,7 +96,7 @@ class Checkpoint8:
         exponent = self.steps.to(torch.int32)
         step = torch.where(exponent == 255, 0x7fc00000, exponent << 23).view(torch.float32)
         values = self.codes.view(2, rows, groups, GROUP).to(torch.float32) * step.unsqueeze(-1)
-        values = values.view(2, rows, groups * GROUP)[:, :, :n_cols].reshape(2, *self.shape)
+        values = values.view(2, rows, groups * GROUP)[:, :, :n_cols].contiguous().view(2, *self.shape)
         return values[0], values[1]
 
 

@@ -12,7 +12,8 @@ ranks take library GEMMs for the adapter terms followed by the streaming SwiGLU 
 are ONE tcgen05 launch (``swiglu_b200_lora_gemm_fwd``, what the reference's v2 attempted in Triton); other
 dtypes and ranks take library GEMMs and the epilogue above, in place over the base projections as in the
 reference's v6.  Backward: library GEMMs around one elementwise pass (``swiglu_b200_bwd_recompute``) that turns
-(dh, e, g) into (h, de, dg).
+(dh, e, g) into (h, de, dg).  ``LoRAMLP`` can keep e and g in 8 bits between the passes (``checkpoint="int8"``), where
+they are the two largest tensors the block saves.
 """
 from __future__ import annotations
 
@@ -21,6 +22,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
+from .checkpoint8 import Checkpoint8, ckpt8_backward_recompute, ckpt8_pack
 from .fused_mlp import _launching
 from .swiglu import _as_float, swiglu_backward_recompute, swiglu_forward
 
@@ -188,19 +190,29 @@ def lora_mlp(X, W_gate, A_gate, B_gate, s_gate, W_up, A_up, B_up, s_up, W_down, 
 class LoRAMLP(torch.autograd.Function):
     """Trainable LoRA MLP: gradients for X and the six adapter matrices, base weights frozen.  Same ``apply``
     arguments and gradient tuple as the reference's ``LoRAMLPv3`` (lora_mlp_kernel_v3.py:259-357), plus an optional
-    fourteenth argument ``activation`` (``"silu"``, ``"gelu_tanh"``, ``"gelu_exact"``) for Gemma-style blocks.  The forward
-    keeps X and the adapter-corrected e, g (not h); the backward recomputes h and overwrites the saved e and g
-    with their gradients, so a graph can be walked once."""
+    fourteenth argument ``activation`` (``"silu"``, ``"gelu_tanh"``, ``"gelu_exact"``) for Gemma-style blocks and an optional
+    fifteenth, ``checkpoint``.  The forward keeps X and the adapter-corrected e, g (not h); the backward recomputes h and
+    overwrites the saved e and g with their gradients, so a graph can be walked once.  With ``checkpoint="int8"`` e and g
+    are kept as 8-bit codes instead (``checkpoint8``: 2.06 bytes for the pair where bf16 takes 4), h and all gradients
+    but that of ``dY`` itself are taken at the values those stand for, and nothing saved is overwritten."""
 
     @staticmethod
     def forward(ctx, X, W_gate, A_gate, B_gate, s_gate, W_up, A_up, B_up, s_up, W_down, A_down, B_down, s_down,
-                activation="silu"):
+                activation="silu", checkpoint=None):
+        if checkpoint not in (None, "int8"):
+            raise ValueError(f"checkpoint must be None or 'int8', got {checkpoint!r}")
         if any(t is None for t in (A_gate, B_gate, A_up, B_up, A_down, B_down)):
             raise ValueError("LoRAMLP differentiates the six adapter matrices: all of them must be given "
                              "(use lora_mlp() for a forward pass with a projection that has no adapter)")
         out, e, g = _lora_mlp_forward(X, W_gate, A_gate, B_gate, s_gate, W_up, A_up, B_up, s_up, W_down, A_down,
                                       B_down, s_down, save_eg=True, activation=activation)
-        ctx.save_for_backward(X, e, g, A_gate, B_gate, A_up, B_up, A_down, B_down)
+        ctx.kept = None
+        if checkpoint == "int8":
+            kept = ckpt8_pack(e, g, activation)
+            ctx.kept = (kept.shape, kept.dtype, activation, 1.0, 1.0)
+            ctx.save_for_backward(X, kept.data, None, A_gate, B_gate, A_up, B_up, A_down, B_down)
+        else:
+            ctx.save_for_backward(X, e, g, A_gate, B_gate, A_up, B_up, A_down, B_down)
         ctx.base_weights = (W_gate, W_up, W_down)
         ctx.scales = (s_gate, s_up, s_down)
         ctx.activation = activation
@@ -218,7 +230,9 @@ class LoRAMLP(torch.autograd.Function):
         dyB = dy @ B_down                                   # [M, r]
         dh = dy @ W_down
         dh.addmm_(dyB, A_down, alpha=s_down)
-        if ctx.activation == "silu":
+        if ctx.kept is not None:
+            h, de, dg = ckpt8_backward_recompute(dh, Checkpoint8._of(e, *ctx.kept))  # dh <- h
+        elif ctx.activation == "silu":
             h, de, dg = swiglu_backward_recompute(dh, e, g)  # in place: dh <- h, e <- de, g <- dg
         else:
             from .geglu import geglu_backward_recompute
@@ -245,4 +259,4 @@ class LoRAMLP(torch.autograd.Function):
         dX.addmm_(deB, A_gate, alpha=s_gate)
         dX.addmm_(dgB, A_up, alpha=s_up)
         return (dX.view_as(X), None, dA_gate, dB_gate, None, None, dA_up, dB_up, None, None, dA_down, dB_down, None,
-                None)
+                None, None)

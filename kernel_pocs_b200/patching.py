@@ -23,6 +23,11 @@ One kernel is added that the reference does not have: ``"fused_gate_up"`` replac
 and the activation by the single tcgen05 kernel of ``fused_mlp`` (SiLU) or ``geglu`` (GELU) when the module's
 projections are plain bias-free bf16 ``nn.Linear`` layers (otherwise the module is left to the next kernel in the
 list).  It is opt-in: ``patch(model, kernels=["fused_gate_up", "swiglu"])`` or ``[..., "geglu"]``.
+
+Three more, opt-in as well, hold the block in fewer bits.  ``"swiglu_ckpt8"`` / ``"geglu_ckpt8"`` route the activation
+through ``checkpoint8``, which keeps gate and up in 8 bits for the backward, and ``"lora_mlp_fused_ckpt8"`` is
+``"lora_mlp_fused"`` with the same; ``"mlp_w4"`` quantises the three projections (plain, bias-free, bf16 or fp16) to 4
+bits when the model is patched and runs the block from those: for generating, forward only.
 """
 from __future__ import annotations
 
@@ -30,6 +35,7 @@ from typing import Callable, Dict, List, Optional
 
 import torch
 
+from .checkpoint8 import geglu_ckpt8, swiglu_ckpt8
 from .fused_mlp import fused_gate_up_swiglu
 from .geglu import FusedGateUpGEGLUFunction, geglu
 from .swiglu import swiglu
@@ -80,25 +86,33 @@ def _gelu_form(module) -> str:
     raise NotImplementedError(f"patch: the geglu kernel cannot infer the GELU variant for hidden_activation={name!r}")
 
 
-def make_swiglu_forward(module) -> Callable:
+def make_swiglu_forward(module, activation=swiglu) -> Callable:
     if _activation_name(module) != "silu":
         raise NotImplementedError(
             f"patch: the swiglu kernel only supports activation='silu', got {_activation_name(module)!r}"
         )
 
     def forward(x):
-        return module.down_proj(swiglu(module.gate_proj(x), module.up_proj(x)))
+        return module.down_proj(activation(module.gate_proj(x), module.up_proj(x)))
 
     return forward
 
 
-def make_geglu_forward(module) -> Callable:
+def make_geglu_forward(module, activation=geglu) -> Callable:
     approximate = _gelu_form(module)
 
     def forward(x):
-        return module.down_proj(geglu(module.gate_proj(x), module.up_proj(x), approximate=approximate))
+        return module.down_proj(activation(module.gate_proj(x), module.up_proj(x), approximate=approximate))
 
     return forward
+
+
+def make_swiglu_ckpt8_forward(module) -> Callable:
+    return make_swiglu_forward(module, swiglu_ckpt8)
+
+
+def make_geglu_ckpt8_forward(module) -> Callable:
+    return make_geglu_forward(module, geglu_ckpt8)
 
 
 def make_fused_gate_up_forward(module) -> Callable:
@@ -174,16 +188,20 @@ def make_lora_mlp_forward(module) -> Callable:
     raise SkipPatch
 
 
-def make_lora_mlp_fused_forward(module) -> Callable:
+def _gated_activation(module) -> str:
+    """The module's activation under the name the fused kernels use; ``SkipPatch`` for any other."""
     act = _activation_name(module)
     if act == "silu":
-        activation = "silu"
-    elif act in GELU_TANH:
-        activation = "gelu_tanh"
-    elif act in GELU_EXACT:
-        activation = "gelu_exact"
-    else:
-        raise SkipPatch
+        return "silu"
+    if act in GELU_TANH:
+        return "gelu_tanh"
+    if act in GELU_EXACT:
+        return "gelu_exact"
+    raise SkipPatch
+
+
+def make_lora_mlp_fused_forward(module, checkpoint=None) -> Callable:
+    activation = _gated_activation(module)
     for proj in (module.gate_proj, module.up_proj, module.down_proj):
         w, a, b, _, _ = _lora_parts(proj)
         # LoRAMLP differentiates the adapters and the input only: the base weights must be frozen
@@ -193,7 +211,10 @@ def make_lora_mlp_fused_forward(module) -> Callable:
 
     # what the block does when its adapters cannot be folded in at call time: route through the (wrapped)
     # projections, as the reference's own patched forward does
-    routed = make_swiglu_forward(module) if activation == "silu" else make_geglu_forward(module)
+    if checkpoint is None:
+        routed = make_swiglu_forward(module) if activation == "silu" else make_geglu_forward(module)
+    else:
+        routed = make_swiglu_ckpt8_forward(module) if activation == "silu" else make_geglu_ckpt8_forward(module)
 
     def forward(x):
         # tensors are looked up at call time: optimiser steps, .to() moves and adapter switches are seen
@@ -204,7 +225,31 @@ def make_lora_mlp_fused_forward(module) -> Callable:
         except SkipPatch:
             # adapters disabled or merged after patch() (e.g. inside PEFT's ``with model.disable_adapter():``)
             return routed(x)
-        return LoRAMLP.apply(x, wg, ag, bg, sg, wu, au, bu, su, wd, ad, bd, sd, activation)
+        return LoRAMLP.apply(x, wg, ag, bg, sg, wu, au, bu, su, wd, ad, bd, sd, activation, checkpoint)
+
+    return forward
+
+
+def make_lora_mlp_fused_ckpt8_forward(module) -> Callable:
+    return make_lora_mlp_fused_forward(module, checkpoint="int8")
+
+
+def make_mlp_w4_forward(module) -> Callable:
+    activation = _gated_activation(module)
+    projections = (module.gate_proj, module.up_proj, module.down_proj)
+    for proj in projections:
+        if (type(proj) is not torch.nn.Linear or proj.bias is not None
+                or proj.weight.dtype not in (torch.bfloat16, torch.float16)):
+            raise SkipPatch
+    from .w4 import quantize_w4, w4_mlp
+
+    # quantised once: later changes of the module's weights are not seen
+    weights = [quantize_w4(proj.weight) for proj in projections]
+
+    def forward(x):
+        if weights[0].device != x.device:
+            weights[:] = [w.to(x.device) for w in weights]
+        return w4_mlp(x, *weights, activation)
 
     return forward
 
@@ -215,6 +260,10 @@ FORWARD_MAKERS: Dict[str, Callable] = {
     "fused_gate_up": make_fused_gate_up_forward,
     "lora_mlp": make_lora_mlp_forward,
     "lora_mlp_fused": make_lora_mlp_fused_forward,
+    "swiglu_ckpt8": make_swiglu_ckpt8_forward,
+    "geglu_ckpt8": make_geglu_ckpt8_forward,
+    "lora_mlp_fused_ckpt8": make_lora_mlp_fused_ckpt8_forward,
+    "mlp_w4": make_mlp_w4_forward,
 }
 
 

@@ -11,9 +11,9 @@ numbers inside the kernel that multiplies them:
     W4Weight(packed, scales, zeros, ...) one from codes that exist already
 
 W[n, k] is ``(code - zero) * scale``; products with x are summed in fp32 and scaled in fp32, and the result is rounded
-once to the dtype of x.  ``MATVEC_ROWS`` tokens and fewer take these kernels; more (a prompt) take the weights written
-out in 16 bits by ``W4Weight.dequantize`` and the tensor-core projections of ``fused_mlp`` / ``geglu``, whose
-operands then carry one more rounding (half a unit of the 16-bit type per weight).  Forward only: weights are frozen and
+once to the dtype of x.  Up to ``LINEAR_ROWS`` / ``GATE_UP_ROWS`` tokens take these kernels; more (a prompt) take the
+weights written out in 16 bits by ``W4Weight.dequantize`` and a library product, or the tensor-core projections of
+``fused_mlp`` / ``geglu``, whose operands then carry one more rounding (half a unit of the 16-bit type per weight).  Forward only: weights are frozen and
 an input that wants a gradient is refused.  The reference has no counterpart (its inference path is bf16,
 kernels/lora_mlp/experiments/v5/lora_mlp_kernel_v5.py:451-454).  There is no path for tensors that are not on a CUDA
 device.
@@ -31,7 +31,10 @@ from .swiglu import _DTYPE_CODE, _stream
 DTYPES = (torch.bfloat16, torch.float16)
 GROUP_SIZES = (32, 64, 128)
 TILE_ROWS, TILE_COLS, CODE_BYTES = 16, 128, 1024
-MATVEC_ROWS = 32
+# Tokens up to which the 4-bit kernels are the faster side, bf16 on B200 (4-bit / 16-bit, us; the 4-bit side reads the
+# weights again for every 32 tokens).  Linear 14336 -> 4096: 35.8 / 53.7 with 64 tokens, 64.0 / 54.9 with 128; 4096 ->
+# 14336: 39.5 / 49.4 and 72.2 / 48.8.  Gate and up 4096 -> 14336: 103.9 / 115.6 with 96, 133.5 / 116.0 with 128.
+LINEAR_ROWS, GATE_UP_ROWS = 64, 96
 
 
 def _ceil(a: int, b: int) -> int:
@@ -246,7 +249,7 @@ def w4_linear(x: torch.Tensor, weight: W4Weight) -> torch.Tensor:
     _check_tokens(x, weight, "w4_linear")
     n, k = weight.out_features, weight.in_features
     m = x.numel() // k
-    if m > MATVEC_ROWS:
+    if m > LINEAR_ROWS:
         return x @ weight.dequantize().t()
     y = x.new_empty((*x.shape[:-1], n))
     x, pitch = _aligned_rows(x)
@@ -289,7 +292,7 @@ def w4_gate_up(x: torch.Tensor, w_gate: W4Weight, w_up: W4Weight, activation: st
     _check_tokens(x, w_gate, "w4_gate_up")
     n, k = w_gate.out_features, w_gate.in_features
     m = x.numel() // k
-    if m > MATVEC_ROWS:
+    if m > GATE_UP_ROWS:
         return _gate_up_16bit(x, w_gate, w_up, activation, gm, dm)
     h = x.new_empty((*x.shape[:-1], n))
     x, pitch = _aligned_rows(x)

@@ -457,3 +457,66 @@ def test_side_stream():
         got = ckpt8_backward(dh, kept)
     side.synchronize()
     assert same_bits(h, want_h) and same_bits(got[0], want[0]) and same_bits(got[1], want[1])
+
+
+# ------------------------------------------------------------------------------------ in the LoRA block
+
+
+def _lora_operands(dtype, m, hidden, inter, r, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def t(*shape, std):
+        return (std * torch.randn(shape, generator=g, device="cuda")).to(dtype)
+
+    W = [t(inter, hidden, std=hidden ** -0.5), t(inter, hidden, std=hidden ** -0.5), t(hidden, inter, std=inter ** -0.5)]
+    A = [t(r, hidden, std=hidden ** -0.5), t(r, hidden, std=hidden ** -0.5), t(r, inter, std=inter ** -0.5)]
+    B = [t(inter, r, std=0.1), t(inter, r, std=0.1), t(hidden, r, std=0.1)]
+    return t(2, m // 2, hidden, std=1.0), W, A, B
+
+
+@gpu
+@pytest.mark.parametrize("activation", ACTS)
+@pytest.mark.parametrize("dtype,r", [(torch.bfloat16, 16), (torch.float32, 5), (torch.float16, 8)])
+def test_lora_mlp_with_8_bit_checkpoints(dtype, r, activation):
+    """The gradients are those of the block's own backward on the kept e and g, bit for bit; the forward is untouched."""
+    from types import SimpleNamespace
+
+    from kernel_pocs_b200.fused_mlp import check_status
+    from kernel_pocs_b200.lora_mlp import LoRAMLP
+
+    X, W, A, B = _lora_operands(dtype, 66, 128, 336, r)
+    leaves = [X, *A, *B]
+    for t in leaves:
+        t.requires_grad_()
+
+    def run(*checkpoint):
+        return LoRAMLP.apply(X, W[0], A[0], B[0], 0.5, W[1], A[1], B[1], 2.0, W[2], A[2], B[2], 1.5, activation,
+                             *checkpoint)
+
+    plain, kept = run(), run("int8")
+    assert same_bits(plain, kept)
+    e, g = plain.grad_fn.saved_tensors[1:3]
+    saved = kept.grad_fn.saved_tensors[1]
+    assert saved.dtype == torch.uint8 and saved.numel() == Checkpoint8.size((66, 336))
+    k = ckpt8_pack(e, g, activation)
+    eh, gh = (t.to(dtype) for t in k.dequantize())
+    dY = torch.randn_like(plain)
+    got = torch.autograd.grad(kept, leaves, dY, retain_graph=True)
+    again = torch.autograd.grad(kept, leaves, dY)            # nothing saved was overwritten
+    ctx = SimpleNamespace(saved_tensors=(X, eh, gh, A[0], B[0], A[1], B[1], A[2], B[2]), base_weights=tuple(W),
+                          scales=(0.5, 2.0, 1.5), activation=activation, kept=None)
+    with torch.no_grad():
+        want = LoRAMLP.backward(ctx, dY)
+    want = [want[i] for i in (0, 2, 6, 10, 3, 7, 11)]
+    for a, b, c in zip(got, want, again):
+        assert same_bits(a, b) and same_bits(a, c)
+    check_status()
+
+
+@gpu
+def test_lora_mlp_refuses_an_unknown_checkpoint():
+    from kernel_pocs_b200.lora_mlp import LoRAMLP
+
+    X, W, A, B = _lora_operands(torch.float32, 4, 16, 32, 4)
+    with pytest.raises(ValueError, match="checkpoint must be"):
+        LoRAMLP.apply(X, W[0], A[0], B[0], 1.0, W[1], A[1], B[1], 1.0, W[2], A[2], B[2], 1.0, "silu", "fp8")

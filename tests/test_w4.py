@@ -213,7 +213,8 @@ def test_c_entries_refuse_bad_arguments_without_a_device():
 
 
 SHAPES = [(1, 1, 1), (1, 16, 128), (2, 17, 129), (1, 4096, 1024), (8, 33, 640), (9, 48, 1000), (16, 100, 384),
-          (17, 64, 257), (32, 131, 2051), (3, 2731, 1000), (1, 31, 14336), (7, 5, 7), (31, 16, 100)]
+          (17, 64, 257), (32, 131, 2051), (3, 2731, 1000), (1, 31, 14336), (7, 5, 7), (31, 16, 100), (33, 40, 640), (64, 129, 300),
+          (2, 70, 9000), (1, 64, 20000)]
 
 
 @gpu
@@ -236,7 +237,8 @@ def test_linear(dtype, group, zeros, m, n, k):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("m,n,k,group,zeros", [(1, 16, 128, 128, False), (1, 2731, 1000, 32, True),
                                                (8, 100, 4096, 64, True), (12, 77, 513, 128, False),
-                                               (32, 40, 2048, 64, False), (5, 3, 9, 32, True)])
+                                               (32, 40, 2048, 64, False), (5, 3, 9, 32, True),
+                                               (96, 130, 260, 64, True), (2, 33, 6000, 128, True)])
 def test_gate_up(act, gm, dm, dtype, m, n, k, group, zeros):
     wg, g64 = make(n, k, group, zeros, dtype, seed=n)
     wu, u64 = make(n, k, group, zeros, dtype, seed=n + 1)
@@ -324,10 +326,10 @@ def test_infinities_and_nan_stay_in_their_token(dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("m,n,k", [(33, 64, 256), (100, 48, 1000), (40, 37, 129)])
+@pytest.mark.parametrize("m,n,k", [(97, 64, 256), (150, 48, 1000), (120, 37, 129)])
 def test_many_tokens_take_the_16_bit_weights(dtype, m, n, k):
-    """Above MATVEC_ROWS every weight is rounded to 16 bits once more: half a unit of each product's magnitude."""
-    assert m > w4.MATVEC_ROWS
+    """Above the limits every weight is rounded to 16 bits once more: half a unit of each product's magnitude."""
+    assert m > max(w4.LINEAR_ROWS, w4.GATE_UP_ROWS)
     w, w64 = make(n, k, 64, True, dtype)
     wu, u64 = make(n, k, 64, False, dtype, seed=9)
     x = tokens(m, k, dtype)
