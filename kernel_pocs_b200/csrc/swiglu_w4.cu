@@ -133,6 +133,17 @@ __device__ __forceinline__ void warp_copy(uint32_t dst, const char* src, int byt
     if ((i * 32 + lane) * 16 < bytes) copy16(dst + (i * 32 + lane) * 16, src + (i * 32 + lane) * 16);
 }
 
+// Launches that follow one another.  A token's projections are launches of a few microseconds in a row, so a launch may
+// start while the last CTAs of the one before it (of this file: no other kernel lets it) are still at work.  Until
+// `wait_for_previous` it touches no memory but to have its first weights brought to L2; from there on everything that
+// was enqueued earlier is complete and visible.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Has `bytes` (a multiple of 16) at `p` brought to L2.
+__device__ __forceinline__ void prefetch_l2(const char* p, int bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
+
 // Clusters.  A launch without one is a cluster of one CTA.
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -173,45 +184,45 @@ constexpr int kTokenBytes = kTileCols * 2;  // a token's part of a column tile
 // ------------------------------------------------------------------ up to 32 tokens: 16-bit products
 
 // Shared memory of a CTA: DEPTH stages of one column tile each, then where the cluster's sums arrive.
-template <int MATS, int RT, int NT, int GROUPS> struct Cfg {
+template <int MATS, int NT, int GROUPS> struct Cfg {
   static constexpr int SLOT = block_bytes(GROUPS, true);
-  static constexpr int WEIGHTS = kWarps * MATS * RT * SLOT, STAGE = WEIGHTS + 8 * NT * kTokenBytes;
-  static constexpr int CTAS = MATS * RT * NT <= 2 ? 3 : 2;  // to an SM
-  static constexpr int OUTPUTS = kWarps * RT * kTileRows * 8 * NT;
+  static constexpr int WEIGHTS = kWarps * MATS * SLOT, STAGE = WEIGHTS + 8 * NT * kTokenBytes;
+  static constexpr int CTAS = 2;  // to an SM
+  static constexpr int OUTPUTS = kWarps * kTileRows * 8 * NT;
   static constexpr int ARRIVALS = MATS * (OUTPUTS + 64) * 4;
   static constexpr int FIT = (220 * 1024 / CTAS - ARRIVALS) / STAGE;
   static constexpr int DEPTH = FIT < 3 ? 3 : FIT > 8 ? 8 : FIT;
   static constexpr int SMEM = DEPTH * STAGE + ARRIVALS;
-  static_assert(MATS * 8 * NT * (kWarps * RT * kTileRows + 4) * 4 <= DEPTH * STAGE,
+  static_assert(MATS * 8 * NT * (kWarps * kTileRows + 4) * 4 <= DEPTH * STAGE,
                 "the sums on their way out reuse the stages");
 };
 
-// A CTA owns 8 * RT row tiles (RT to a warp) of MATS matrices, 8 * NT tokens and, as rank r of a cluster of `split`
+// A CTA owns 8 row tiles (one to a warp; two would read the tokens' fragments once for both, but 128 rows to a CTA
+// balance better: fp16 32 x 5504 -> 11009 21.6 us against 23.5) of MATS matrices, 8 * NT tokens and, as rank r of a cluster of `split`
 // CTAs, the r-th part of the column tiles.  Each rank finishes a slice of the outputs: the others store their sums for
 // it into its shared memory, where they are added in a fixed order.
-template <class T, int MATS, int RT, int NT, int GROUPS>
-__global__ void __launch_bounds__(32 * kWarps, Cfg<MATS, RT, NT, GROUPS>::CTAS)
+template <class T, int MATS, int NT, int GROUPS>
+__global__ void __launch_bounds__(32 * kWarps, Cfg<MATS, NT, GROUPS>::CTAS)
 w4_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, int activation, float gm, float dm) {
   using H = Half2<T>;
-  using C = Cfg<MATS, RT, NT, GROUPS>;
+  using C = Cfg<MATS, NT, GROUPS>;
   constexpr int DEPTH = C::DEPTH, PIECES = 8 * NT * 16, ROUNDS = (PIECES + 32 * kWarps - 1) / (32 * kWarps);
   extern __shared__ __align__(16) unsigned char smem[];
   cluster_arrive();  // all CTAs of the cluster have started once this is waited for
+  let_next_start();
   const uint32_t smem_addr = (uint32_t)__cvta_generic_to_shared(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int rank = (int)cluster_rank(), split = s.split;
   const int row_tiles = (int)((s.n + kTileRows - 1) / kTileRows);
-  const int row_tile0 = (int)cluster_index() * (kWarps * RT), row_tile = row_tile0 + warp * RT;  // of the CTA, the warp
+  const int row_tile0 = (int)cluster_index() * kWarps, row_tile = row_tile0 + warp;  // of the CTA, the warp
   const long long token0 = (long long)blockIdx.y * (8 * NT);
   const int first = rank * s.share + min(rank, s.over), last = first + s.share + (rank < s.over ? 1 : 0);
   const W4 w[2] = {w0, w1};
 
-  const char* src[MATS][RT];  // the warp's next block of each row tile
+  const char* src[MATS];  // the warp's next block
 #pragma unroll
   for (int a = 0; a < MATS; ++a)
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-      src[a][r] = cbyte(w[a].blocks) + ((long long)(row_tile + r) * s.col_tiles + first) * block_bytes(GROUPS, w[a].zeros);
+    src[a] = cbyte(w[a].blocks) + ((long long)row_tile * s.col_tiles + first) * block_bytes(GROUPS, w[a].zeros);
   const char* x_src[ROUNDS];  // this thread's pieces of 8 columns of a token, and how many bytes of the row are left there
   long long x_left[ROUNDS];
 #pragma unroll
@@ -228,14 +239,11 @@ w4_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, int acti
     if (c < last) {
       const uint32_t stage = smem_addr + fill;
 #pragma unroll
-      for (int a = 0; a < MATS; ++a)
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          const int bytes = block_bytes(GROUPS, w[a].zeros);
-          if (row_tile + r < row_tiles)
-            warp_copy<(C::SLOT + 511) / 512>(stage + ((warp * MATS + a) * RT + r) * C::SLOT, src[a][r], bytes, lane);
-          src[a][r] += bytes;
-        }
+      for (int a = 0; a < MATS; ++a) {
+        const int bytes = block_bytes(GROUPS, w[a].zeros);
+        if (row_tile < row_tiles) warp_copy<(C::SLOT + 511) / 512>(stage + (warp * MATS + a) * C::SLOT, src[a], bytes, lane);
+        src[a] += bytes;
+      }
       // tokens: every other one has its 64-byte quarters swapped in pairs, so that the 8 lanes that read together (two
       // tokens, four pieces) touch all 32 banks
 #pragma unroll
@@ -252,10 +260,16 @@ w4_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, int acti
     fill = fill == (DEPTH - 1) * C::STAGE ? 0 : fill + C::STAGE;
   };
 
+  if (lane < MATS && row_tile < row_tiles) {
+    const W4& mine = lane == 0 ? w0 : w1;
+    const int bytes = block_bytes(GROUPS, mine.zeros);
+    prefetch_l2(cbyte(mine.blocks) + ((long long)row_tile * s.col_tiles + first) * bytes, min(DEPTH - 1, last - first) * bytes);
+  }
+  wait_for_previous();
 #pragma unroll 1
   for (int i = 0; i < DEPTH - 1; ++i) fetch(first + i);
 
-  float acc[MATS * RT][NT][4] = {};
+  float acc[MATS][NT][4] = {};
   int take = 0;  // offset of the stage to read next
 #pragma unroll 1
   for (int c = first; c < last; ++c) {
@@ -264,14 +278,14 @@ w4_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, int acti
     fetch(c + DEPTH - 1);
     const unsigned char* stage = smem + take;
     take = take == (DEPTH - 1) * C::STAGE ? 0 : take + C::STAGE;
-    uint4 codes[MATS * RT][2];
+    uint4 codes[MATS][2];
 #pragma unroll
-    for (int q = 0; q < MATS * RT; ++q)
+    for (int q = 0; q < MATS; ++q)
 #pragma unroll
       for (int hi = 0; hi < 2; ++hi)
-        codes[q][hi] = *reinterpret_cast<const uint4*>(stage + (warp * MATS * RT + q) * C::SLOT + hi * 512 + lane * 16);
-    float part[MATS * RT][NT][4];
-    uint32_t bias[MATS * RT][2];
+        codes[q][hi] = *reinterpret_cast<const uint4*>(stage + (warp * MATS + q) * C::SLOT + hi * 512 + lane * 16);
+    float part[MATS][NT][4];
+    uint32_t bias[MATS][2];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       constexpr int per_group = 4 / GROUPS;  // words per group
@@ -282,11 +296,11 @@ w4_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, int acti
         b[j] = *reinterpret_cast<const uint4*>(stage + C::WEIGHTS + (8 * j + g) * kTokenBytes +
                                                ((4 * u + t) ^ ((g & 1) << 2)) * 16);
 #pragma unroll
-      for (int q = 0; q < MATS * RT; ++q) {
-        const unsigned char* tail = stage + (warp * MATS * RT + q) * C::SLOT + kTileBytes;
+      for (int q = 0; q < MATS; ++q) {
+        const unsigned char* tail = stage + (warp * MATS + q) * C::SLOT + kTileBytes;
         if (u % per_group == 0) {
           bias[q][0] = bias[q][1] = H::pair(-8.0f * H::kUnit);
-          if (w[q / RT].zeros) {
+          if (w[q].zeros) {
             const uint32_t z = *reinterpret_cast<const uint16_t*>(tail + GROUPS * 32 + at);
             bias[q][0] = H::pair(-H::kUnit * zero_point(z & 0xffu));
             bias[q][1] = H::pair(-H::kUnit * zero_point(z >> 8));
@@ -326,16 +340,16 @@ w4_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, int acti
 
   copies_wait<0>();
   __syncthreads();  // the stages are done with
-  constexpr int kRows = kWarps * RT * kTileRows, OUTPUTS = C::OUTPUTS;
+  constexpr int kRows = kWarps * kTileRows, OUTPUTS = C::OUTPUTS;
   constexpr int kPitch = kRows + 4, kMatrix = 8 * NT * kPitch;  // four tokens of a warp's store hit different banks
   float* sums = reinterpret_cast<float*>(smem);                 // [matrix][token][row]
 #pragma unroll
-  for (int q = 0; q < MATS * RT; ++q)
+  for (int q = 0; q < MATS; ++q)
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e)  // row g + 8 (e / 2), token 2t + e % 2 of a tile
-        sums[q / RT * kMatrix + (8 * j + 2 * t + e % 2) * kPitch + (warp * RT + q % RT) * kTileRows + g + 8 * (e / 2)] =
+        sums[q * kMatrix + (8 * j + 2 * t + e % 2) * kPitch + warp * kTileRows + g + 8 * (e / 2)] =
             acc[q][j][e] * (1.0f / H::kUnit);
   __syncthreads();
 
@@ -454,6 +468,7 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
   constexpr int DEPTH = C::DEPTH;
   extern __shared__ __align__(16) unsigned char smem[];
   cluster_arrive();  // all CTAs of the cluster have started once this is waited for
+  let_next_start();
   const uint32_t smem_addr = (uint32_t)__cvta_generic_to_shared(smem);
   unsigned char* digits = smem + C::RING;
   float* digit_sums = reinterpret_cast<float*>(digits + C::DIGITS);
@@ -548,6 +563,14 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
     fill = fill == (DEPTH - 1) * C::PAIR ? 0 : fill + C::PAIR;
   };
 
+  if (lane < MATS && there && first < last) {
+    const W4& mine = lane == 0 ? w0 : w1;
+    const int bytes = block_bytes(GROUPS, mine.zeros);
+    // both column warps of a row ask for the same few pairs
+    prefetch_l2(cbyte(mine.blocks) + ((long long)row_tile * s.col_tiles + 2 * first) * bytes,
+                min((DEPTH - 1) * kColWarps * 2, min(2 * last, s.col_tiles) - 2 * first) * bytes);
+  }
+  wait_for_previous();
   Vec<16> token = read_token(first, 0);
 #pragma unroll 1
   for (int i = 0; i < DEPTH - 1; ++i) fetch(first + col_warp + i * kColWarps);
@@ -800,14 +823,17 @@ int start(void (*kernel)(P...), Launcher& known, long long clusters, long long g
     if (e == cudaSuccess && dev < 64) known.opted_in.fetch_or(1ULL << dev, std::memory_order_relaxed);
   }
   if (e != cudaSuccess) return note_cuda_error(SWIGLU_B200_ERR_DEVICE, e);
-  cudaLaunchAttribute cluster{};
+  cudaLaunchAttribute attrs[2] = {};
+  cudaLaunchAttribute& cluster = attrs[0];
   cluster.id = cudaLaunchAttributeClusterDimension;
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
   cfg.blockDim = dim3(32 * kWarps);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = st;
-  cfg.attrs = &cluster;
+  cfg.attrs = attrs;
   cfg.numAttrs = 1;
   int split = parts < 8 ? parts : 8;
   for (; split > 1; --split) {
@@ -827,6 +853,7 @@ int start(void (*kernel)(P...), Launcher& known, long long clusters, long long g
   s.slice = (outputs + unit * split - 1) / (unit * split) * unit;
   cluster.val.clusterDim.x = (unsigned)split;
   cfg.gridDim = dim3((unsigned)(clusters * split), (unsigned)gy);
+  cfg.numAttrs = 2;
   e = cudaLaunchKernelEx(&cfg, kernel, y, x, w0, w1, s, activation, gm, dm);
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -838,13 +865,11 @@ int start(void (*kernel)(P...), Launcher& known, long long clusters, long long g
 
 template <class T, int MATS, int NT, int GROUPS>
 int launch(void* y, const void* x, const W4* w, const W4Shape& s, int activation, float gm, float dm, cudaStream_t st) {
-  // Two weight tiles to a warp where 32 tokens are read beside them: the fragments of those are 8 KB per column tile,
-  // 8 times the codes of one tile.
-  constexpr int RT = NT == 4 && MATS == 1 ? 2 : 1, kRows = kWarps * RT * kTileRows;
+  constexpr int kRows = kWarps * kTileRows;
   static Launcher known;
-  return start(w4_kernel<T, MATS, RT, NT, GROUPS>, known, (s.n + kRows - 1) / kRows, (s.m + 8 * NT - 1) / (8 * NT),
-               s.col_tiles, kRows * (int)(s.m < 8 * NT ? s.m : 8 * NT), 4, Cfg<MATS, RT, NT, GROUPS>::SMEM, st, y, x,
-               w[0], w[MATS - 1], s, activation, gm, dm);
+  return start(w4_kernel<T, MATS, NT, GROUPS>, known, (s.n + kRows - 1) / kRows, (s.m + 8 * NT - 1) / (8 * NT),
+               s.col_tiles, kRows * (int)(s.m < 8 * NT ? s.m : 8 * NT), 4, Cfg<MATS, NT, GROUPS>::SMEM, st, y, x, w[0],
+               w[MATS - 1], s, activation, gm, dm);
 }
 
 template <class T, int MATS, int GROUPS>
@@ -886,6 +911,7 @@ int run(void* y, const void* x, const W4* w, W4Shape s, int64_t m, int64_t x_row
       if (m <= kDigitTokens) return launch_digits<T, MATS, G>(y, x, w, s, activation, gm, dm, st);
       if (m <= 8) return launch<T, MATS, 1, G>(y, x, w, s, activation, gm, dm, st);
       if (m <= 16) return launch<T, MATS, 2, G>(y, x, w, s, activation, gm, dm, st);
+      if (m <= 24) return launch<T, MATS, 3, G>(y, x, w, s, activation, gm, dm, st);
       return launch<T, MATS, 4, G>(y, x, w, s, activation, gm, dm, st);
     };
     if (s.groups_log2 == 0) return grouped(std::integral_constant<int, 1>{});

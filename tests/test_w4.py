@@ -403,3 +403,39 @@ def test_captured_token_replays_on_new_inputs_and_streams():
         torch.cuda.synchronize()
         want = w4_mlp(x, w, wu, wd)
         assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
+@gpu
+@pytest.mark.parametrize("m", [1, 2, 8, 24])
+def test_launches_in_a_row_see_what_came_before_them(m):
+    """Launches may start before the one in front of them has ended: tokens, weights and outputs that change from one
+    call to the next, with nothing waited for in between, against the same calls one at a time."""
+    dtype = torch.bfloat16
+    w, _ = make(700, 512, 64, True, dtype)
+    wu, _ = make(700, 512, 64, False, dtype, seed=5)
+    wd, _ = make(512, 700, 128, True, dtype, seed=6)
+    others = [make(700, 512, 64, True, dtype, seed=20 + i)[0].blocks for i in range(3)]
+    start = tokens(m, 512, dtype)
+
+    def chain(wait):
+        x, seen = start.clone(), []
+        for i in range(40):
+            if i % 5 == 0:
+                w.blocks.copy_(others[i // 5 % 3])        # new weights, enqueued right before they are read
+            h = w4_gate_up(x, w, wu)
+            if wait:
+                torch.cuda.synchronize()
+            y = w4_linear(h, wd)
+            if wait:
+                torch.cuda.synchronize()
+            x.copy_(y / y.float().abs().amax(dim=1, keepdim=True).clamp(min=1e-20).to(dtype))
+            seen += [y, h.clone()]
+            del h
+        return torch.stack([t.float().sum() for t in seen]), seen
+
+    sums, want = chain(True)
+    for _ in range(3):
+        again, got = chain(False)
+        torch.cuda.synchronize()
+        assert bool(torch.isfinite(sums).all()) and torch.equal(again, sums)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
