@@ -111,6 +111,7 @@ struct Place {
   bool full;     // all EPV columns exist
   int rest;      // columns of a partial frame, 0 for any other
   bool first, last;  // no full frame of the same task before / after this one
+  bool whole;        // every lane of the task has a full frame (uniform over the warp)
   __device__ __forceinline__ explicit Place(const Ckpt8Shape& s) {
     const int lane = threadIdx.x & 31;
     const int task = (int)blockIdx.x * (int)(blockDim.x >> 5) + (int)(threadIdx.x >> 5);
@@ -122,60 +123,83 @@ struct Place {
     rest = v == n_full ? (int)(s.cols % EPV) : 0;
     first = lane == 0;
     last = lane == 31 || v == n_full - 1;
+    whole = (long long)task * 32 + 32 <= n_full;
   }
 };
 
-// The lane's frame of a row that starts at `row`; columns that do not exist read as zero.
-template <class T, bool SKEW, int LDM>
-__device__ __forceinline__ void frame_issue(const char* row, const Place<T>& at, Window& w) {
-  if constexpr (!SKEW) {
-    if (at.full) w.main = Ld<32, LDM>::ld(row + at.v * 32);
-    else w.main = Vec<32>{};
-  } else {
-    const int s = (int)((uintptr_t)row & 31);
-    w.main = Vec<32>{};
-    w.nb = Vec<16>{};
-    ld_window_issue<LDM>(row, at.v, s, at.full, w);
-  }
-}
-template <class T, bool SKEW>
-__device__ __forceinline__ Vec<32> frame_finish(const char* row, const Place<T>& at, const Window& w) {
-  if constexpr (!SKEW) {
-    return w.main;
-  } else {
-    constexpr int ES = (int)sizeof(T);
-    Vec<32> v = ld_window_finish(w, (int)((uintptr_t)row & 31));  // zero where nothing was loaded
-    if (at.rest) {
-      const char* p = row + at.v * 32;
-#pragma unroll
-      for (int e = 0; e < Place<T>::EPV; ++e)
-        if (e < at.rest) {
-          const uint32_t x = Ld<ES, LD_PLAIN>::ld(p + e * ES).w[0];
-          v.w[e * ES / 4] |= (e * ES % 4) ? x << 16 : x;
-        }
+// The lane's frame of a row that starts at `row`; columns that do not exist read as zero.  In a WHOLE task every lane
+// has a full frame, which it reads as the two or three aligned 16-byte pieces it lies in.
+struct Pieces {
+  Vec<16> p[3];
+};
+template <class T, bool SKEW, bool WHOLE> struct Frame {
+  Window w;
+  Pieces q;
+
+  template <int LDM> __device__ __forceinline__ void issue(const char* row, const Place<T>& at) {
+    if constexpr (WHOLE && !SKEW) {
+      w.main = Ld<32, LDM>::ld(row + at.v * 32);
+    } else if constexpr (WHOLE) {
+      const char* p = row + at.v * 32 - ((uintptr_t)row & 15);
+      q.p[0] = Ld<16, LDM>::ld(p);
+      q.p[1] = Ld<16, LDM>::ld(p + 16);
+      q.p[2] = ((uintptr_t)row & 15) ? Ld<16, LDM>::ld(p + 32) : q.p[1];
+    } else if constexpr (!SKEW) {
+      if (at.full) w.main = Ld<32, LDM>::ld(row + at.v * 32);
+      else w.main = Vec<32>{};
+    } else {
+      w.main = Vec<32>{};
+      w.nb = Vec<16>{};
+      ld_window_issue<LDM>(row, at.v, (int)((uintptr_t)row & 31), at.full, w);
     }
-    return v;
   }
-}
+  __device__ __forceinline__ Vec<32> finish(const char* row, const Place<T>& at) const {
+    if constexpr (!SKEW) {
+      return w.main;
+    } else if constexpr (WHOLE) {
+      const uint32_t x[12] = {q.p[0].w[0], q.p[0].w[1], q.p[0].w[2], q.p[0].w[3], q.p[1].w[0], q.p[1].w[1],
+                              q.p[1].w[2], q.p[1].w[3], q.p[2].w[0], q.p[2].w[1], q.p[2].w[2], q.p[2].w[3]};
+      return shift_window(x, (int)((uintptr_t)row & 15));
+    } else {
+      constexpr int ES = (int)sizeof(T);
+      Vec<32> v = ld_window_finish(w, (int)((uintptr_t)row & 31));  // zero where nothing was loaded
+      if (at.rest) {
+        const char* p = row + at.v * 32;
+#pragma unroll
+        for (int e = 0; e < Place<T>::EPV; ++e)
+          if (e < at.rest) {
+            const uint32_t x = Ld<ES, LD_PLAIN>::ld(p + e * ES).w[0];
+            v.w[e * ES / 4] |= (e * ES % 4) ? x << 16 : x;
+          }
+      }
+      return v;
+    }
+  }
+};
 
 // Stores the lane's frame into a row that starts at `row`.  All 32 lanes call this together.
-template <class T, bool SKEW>
+template <class T, bool SKEW, bool WHOLE>
 __device__ __forceinline__ void frame_store(char* row, const Place<T>& at, const Vec<32>& v) {
   if constexpr (!SKEW) {
-    if (at.full) St<32, ST_CS>::st(row + at.v * 32, v);
+    if (WHOLE || at.full) St<32, ST_CS>::st(row + at.v * 32, v);
   } else {
     constexpr int ES = (int)sizeof(T);
     char* p = row + at.v * 32;
-    st_skewed32<ST_CS>(p, v, (int)((uintptr_t)row & 31), at.full, at.first, at.last);
-    if (at.rest) {
+    if constexpr (WHOLE) {
+      const int lane = threadIdx.x & 31;
+      st_skewed32<ST_CS>(p, v, (int)((uintptr_t)row & 31), true, lane == 0, lane == 31);
+    } else {
+      st_skewed32<ST_CS>(p, v, (int)((uintptr_t)row & 31), at.full, at.first, at.last);
+      if (at.rest) {
 #pragma unroll
-      for (int e = 0; e < Place<T>::EPV; ++e)
-        if (e < at.rest) {
-          Vec<ES> x;
-          x.w[0] = (e * ES % 4) ? v.w[e * ES / 4] >> 16 : v.w[e * ES / 4];
-          if constexpr (ES == 2) x.w[0] &= 0xffffu;
-          St<ES, ST_PLAIN>::st(p + e * ES, x);
-        }
+        for (int e = 0; e < Place<T>::EPV; ++e)
+          if (e < at.rest) {
+            Vec<ES> x;
+            x.w[0] = (e * ES % 4) ? v.w[e * ES / 4] >> 16 : v.w[e * ES / 4];
+            if constexpr (ES == 2) x.w[0] &= 0xffffu;
+            St<ES, ST_PLAIN>::st(p + e * ES, x);
+          }
+      }
     }
   }
 }
@@ -189,11 +213,11 @@ __device__ __forceinline__ uint32_t group_exponent(const Vec<32>& v) {
   return step_exponent(top);
 }
 
-template <class T>
+template <class T, bool WHOLE>
 __device__ __forceinline__ void codes_store(void* codes, void* steps, const Ckpt8Shape& s, const Place<T>& at,
                                             const float* f, uint32_t e) {
   constexpr int EPV = Place<T>::EPV;
-  if (!at.in_row) return;
+  if (!WHOLE && !at.in_row) return;
   Vec<EPV> c;
   encode<EPV>(f, e, c.w);
   St<EPV, ST_CS>::st(byte(codes) + at.row * s.groups * kGroup + at.v * EPV, c);
@@ -205,10 +229,10 @@ __device__ __forceinline__ void codes_store(void* codes, void* steps, const Ckpt
   }
 }
 
-template <class T>
+template <class T, bool WHOLE>
 __device__ __forceinline__ uint32_t step_load(const void* steps, const Ckpt8Shape& s, const Place<T>& at) {
   uint32_t e = 1;
-  if (at.in_row)
+  if (WHOLE || at.in_row)
     asm volatile("ld.global.nc.u8 %0, [%1];"
                  : "=r"(e) : "l"(cbyte(steps) + at.row * s.groups + at.v / (kGroup / Place<T>::EPV)));
   return e;
@@ -216,66 +240,68 @@ __device__ __forceinline__ uint32_t step_load(const void* steps, const Ckpt8Shap
 
 constexpr int kWarps = 4;  // most warps of a CTA
 
-// CTAs to an SM that the registers are budgeted for (bf16 [16384, 14336], 6 / 8 / 10 / 16 of them: forward 283 / 276 / 277 /
-// 304 us; backward with 6 / 8 / 10 / 12: 385 / 301 / 289 / 292 us, at half-width 11009 packed 103 / 90 / 77 / 78 us; with h
-// 385 / 359 / 357 / 445 us, where GELU loses 3 % from 8 to 10 and the skewed form gains 4 %).
-constexpr int kForwardCtas = 10, kBackwardCtas = 10, kBackwardHCtas = 8;
+// CTAs to an SM that the registers are budgeted for.  bf16 [16384, 14336], 6 / 8 / 10 / 16 of them: forward 283 / 276 / 277 /
+// 304 us; backward with 6 / 8 / 10 / 12: 385 / 301 / 289 / 292 us, and at half-width 11009 packed 103 / 90 / 77 / 78 us.
+constexpr int kCtas = 10;
 
-// h may be NULL: the codes alone are stored.
-template <class T, int ACT, bool SKEW>
-__global__ void __launch_bounds__(32 * kWarps, kForwardCtas)
-ckpt8_fwd_kernel(void* h, void* gate_codes, void* up_codes, void* gate_steps, void* up_steps,
-                 const void* __restrict__ gate, const void* __restrict__ up, Ckpt8Shape s, float gm, float dm) {
+template <class T, int ACT, bool SKEW, bool WHOLE>
+__device__ __forceinline__ void forward_task(void* h, void* gate_codes, void* up_codes, void* gate_steps, void* up_steps,
+                                             const void* gate, const void* up, const Ckpt8Shape& s, const Place<T>& at,
+                                             float gm, float dm) {
   constexpr bool FAST = (sizeof(T) == 2);
   constexpr int EPV = Place<T>::EPV;
-  const Place<T> at(s);
-  if (at.row >= s.rows) return;
   const Consts c(gm, dm);
   const char* gate_row = cbyte(gate) + at.row * s.pitch_in;
   const char* up_row = cbyte(up) + at.row * s.pitch_in;
-  Window wg, wu;
-  frame_issue<T, SKEW, LD_PLAIN>(gate_row, at, wg);
-  frame_issue<T, SKEW, LD_PLAIN>(up_row, at, wu);
-  const Vec<32> vg = frame_finish<T, SKEW>(gate_row, at, wg), vu = frame_finish<T, SKEW>(up_row, at, wu);
+  Frame<T, SKEW, WHOLE> wg, wu;
+  wg.template issue<LD_PLAIN>(gate_row, at);
+  wu.template issue<LD_PLAIN>(up_row, at);
+  const Vec<32> vg = wg.finish(gate_row, at), vu = wu.finish(up_row, at);
   const uint32_t eg = group_exponent<T>(vg), eu = group_exponent<T>(vu);
   float fg[EPV], fu[EPV];
   Codec<T>::template unpack<32>(vg, fg);
   Codec<T>::template unpack<32>(vu, fu);
-  codes_store<T>(gate_codes, gate_steps, s, at, fg, eg);
-  codes_store<T>(up_codes, up_steps, s, at, fu, eu);
+  codes_store<T, WHOLE>(gate_codes, gate_steps, s, at, fg, eg);
+  codes_store<T, WHOLE>(up_codes, up_steps, s, at, fu, eu);
   if (h != nullptr) {
     float fh[EPV];
 #pragma unroll
     for (int i = 0; i < EPV; ++i) fh[i] = Math<FAST, ACT>::fwd(fg[i], fu[i], c);
     Vec<32> vh;
     Codec<T>::template pack<32>(fh, vh);
-    frame_store<T, SKEW>(byte(h) + at.row * s.pitch_out, at, vh);
+    frame_store<T, SKEW, WHOLE>(byte(h) + at.row * s.pitch_out, at, vh);
   }
 }
 
-// With H, h = act(gate*gm) * up * dm of the kept values is stored too; it may overwrite dout (a warp stores only
-// elements whose values its own lanes have read by then).
-template <class T, int ACT, bool SKEW, bool H>
-__global__ void __launch_bounds__(32 * kWarps, H && !SKEW ? kBackwardHCtas : kBackwardCtas)
-ckpt8_bwd_kernel(void* h, void* dgate, void* dup, const void* dout, const void* __restrict__ gate_codes,
-                 const void* __restrict__ up_codes, const void* __restrict__ gate_steps,
-                 const void* __restrict__ up_steps, Ckpt8Shape s, float gm, float dm) {
-  constexpr bool FAST = (sizeof(T) == 2);
-  constexpr int EPV = Place<T>::EPV;
+// h may be NULL: the codes alone are stored.  Tasks without a row's end take a copy of the code that has no predicates.
+template <class T, int ACT, bool SKEW>
+__global__ void __launch_bounds__(32 * kWarps, kCtas)
+ckpt8_fwd_kernel(void* h, void* gate_codes, void* up_codes, void* gate_steps, void* up_steps,
+                 const void* __restrict__ gate, const void* __restrict__ up, Ckpt8Shape s, float gm, float dm) {
   const Place<T> at(s);
   if (at.row >= s.rows) return;
+  if (at.whole) forward_task<T, ACT, SKEW, true>(h, gate_codes, up_codes, gate_steps, up_steps, gate, up, s, at, gm, dm);
+  else forward_task<T, ACT, SKEW, false>(h, gate_codes, up_codes, gate_steps, up_steps, gate, up, s, at, gm, dm);
+}
+
+template <class T, int ACT, bool SKEW, bool H, bool WHOLE>
+__device__ __forceinline__ void backward_task(void* h, void* dgate, void* dup, const void* dout, const void* gate_codes,
+                                              const void* up_codes, const void* gate_steps, const void* up_steps,
+                                              const Ckpt8Shape& s, const Place<T>& at, float gm, float dm) {
+  constexpr bool FAST = (sizeof(T) == 2);
+  constexpr int EPV = Place<T>::EPV;
   const Consts c(gm, dm);
   const char* dout_row = cbyte(dout) + at.row * s.pitch_in;
-  Window wd;
-  frame_issue<T, SKEW, LD_PLAIN>(dout_row, at, wd);
+  Frame<T, SKEW, WHOLE> wd;
+  wd.template issue<LD_PLAIN>(dout_row, at);
   Vec<EPV> cg{}, cu{};
-  if (at.in_row) {
+  if (WHOLE || at.in_row) {
     const long long off = at.row * s.groups * kGroup + at.v * EPV;
     cg = Ld<EPV, LD_NC_NOALLOC>::ld(cbyte(gate_codes) + off);
     cu = Ld<EPV, LD_NC_NOALLOC>::ld(cbyte(up_codes) + off);
   }
-  const uint32_t eg = step_load<T>(gate_steps, s, at), eu = step_load<T>(up_steps, s, at);
-  const Vec<32> vd = frame_finish<T, SKEW>(dout_row, at, wd);
+  const uint32_t eg = step_load<T, WHOLE>(gate_steps, s, at), eu = step_load<T, WHOLE>(up_steps, s, at);
+  const Vec<32> vd = wd.finish(dout_row, at);
   float fg[EPV], fu[EPV], fd[EPV], fdg[EPV], fdu[EPV], fh[EPV];
   decode<EPV / 4>(cg.w, eg, fg);
   decode<EPV / 4>(cu.w, eu, fu);
@@ -287,13 +313,30 @@ ckpt8_bwd_kernel(void* h, void* dgate, void* dup, const void* dout, const void* 
   }
   Vec<32> x;
   Codec<T>::template pack<32>(fdg, x);
-  frame_store<T, SKEW>(byte(dgate) + at.row * s.pitch_grad, at, x);
+  frame_store<T, SKEW, WHOLE>(byte(dgate) + at.row * s.pitch_grad, at, x);
   Codec<T>::template pack<32>(fdu, x);
-  frame_store<T, SKEW>(byte(dup) + at.row * s.pitch_grad, at, x);
+  frame_store<T, SKEW, WHOLE>(byte(dup) + at.row * s.pitch_grad, at, x);
   if constexpr (H) {
     Codec<T>::template pack<32>(fh, x);
-    frame_store<T, SKEW>(byte(h) + at.row * s.pitch_out, at, x);
+    frame_store<T, SKEW, WHOLE>(byte(h) + at.row * s.pitch_out, at, x);
   }
+}
+
+// With H, h = act(gate*gm) * up * dm of the kept values is stored too; it may overwrite dout (a warp stores only
+// elements whose values its own lanes have read by then).  The copy of the code for whole tasks pays for aligned rows
+// (289 -> 276 us); the skewed form is issue-bound and twice its size overflows the instruction cache (with h, half-width
+// 11009 packed: 105 -> 133 us), so it has one copy.
+template <class T, int ACT, bool SKEW, bool H>
+__global__ void __launch_bounds__(32 * kWarps, kCtas)
+ckpt8_bwd_kernel(void* h, void* dgate, void* dup, const void* dout, const void* __restrict__ gate_codes,
+                 const void* __restrict__ up_codes, const void* __restrict__ gate_steps,
+                 const void* __restrict__ up_steps, Ckpt8Shape s, float gm, float dm) {
+  const Place<T> at(s);
+  if (at.row >= s.rows) return;
+  if (!SKEW && at.whole)
+    backward_task<T, ACT, SKEW, H, !SKEW>(h, dgate, dup, dout, gate_codes, up_codes, gate_steps, up_steps, s, at, gm, dm);
+  else
+    backward_task<T, ACT, SKEW, H, false>(h, dgate, dup, dout, gate_codes, up_codes, gate_steps, up_steps, s, at, gm, dm);
 }
 
 // ------------------------------------------------------------------ host side
