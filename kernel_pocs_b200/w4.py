@@ -32,8 +32,8 @@ DTYPES = (torch.bfloat16, torch.float16)
 GROUP_SIZES = (32, 64, 128)
 TILE_ROWS, TILE_COLS, CODE_BYTES = 16, 128, 1024
 # Tokens up to which the 4-bit kernels are the faster side, bf16 on B200 (4-bit / 16-bit, us; the 4-bit side reads the
-# weights again for every 32 tokens).  Linear 14336 -> 4096: 35.8 / 53.7 with 64 tokens, 64.0 / 54.9 with 128; 4096 ->
-# 14336: 39.5 / 49.4 and 72.2 / 48.8.  Gate and up 4096 -> 14336: 103.9 / 115.6 with 96, 133.5 / 116.0 with 128.
+# weights again for every 32 tokens).  Linear 14336 -> 4096: 36.0 / 54.8 with 64 tokens, 67.7 / 55.3 with 96; 4096 ->
+# 14336: 39.9 / 49.6 and 58.7 / 50.4.  Gate and up 4096 -> 14336: 102.4 / 116.4 with 96, 131.0 / 115.9 with 128.
 LINEAR_ROWS, GATE_UP_ROWS = 64, 96
 
 

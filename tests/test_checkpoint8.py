@@ -446,6 +446,30 @@ def test_captured_step_replays_on_new_inputs():
 
 
 @gpu
+def test_captured_autograd_step():
+    """Forward and gradients through autograd in one graph, the leaves made on the capturing stream."""
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        gate, up, dh = inputs(48, 321, torch.float16, seed=1)
+        gate.requires_grad_(), up.requires_grad_()
+        for _ in range(2):
+            torch.autograd.grad(geglu_ckpt8(gate, up), (gate, up), dh)
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        h = geglu_ckpt8(gate, up)
+        grads = torch.autograd.grad(h, (gate, up), dh)
+    with torch.no_grad():
+        for dst, src in zip((gate, up, dh), inputs(48, 321, torch.float16, seed=2)):
+            dst.copy_(src)
+    graph.replay()
+    torch.cuda.synchronize()
+    h0, kept = ckpt8_forward(gate.detach(), up.detach(), "gelu_tanh")
+    want = ckpt8_backward(dh, kept)
+    assert same_bits(h.detach(), h0) and same_bits(grads[0], want[0]) and same_bits(grads[1], want[1])
+
+
+@gpu
 def test_side_stream():
     gate, up, dh = inputs(256, 2048, torch.float16, seed=4)
     want_h, kept = ckpt8_forward(gate, up)
