@@ -17,7 +17,8 @@
  * queried or set on their first launch there; per device, once swiglu_b200_host_fwd_bwd has been
  * called for it, two copy streams and ten events that every later call of that entry point on the
  * device reuses (never destroyed; calls for one device are serialised on the host while they
- * enqueue); and the status array of swiglu_b200_gemm_fwd_noalloc described at its declaration.
+ * enqueue); per device and kernel of swiglu_b200_w4_linear / _gate_up, the shared-memory opt-in and how many clusters
+ * of each size run at once; and the status array of swiglu_b200_gemm_fwd_noalloc described at its declaration.
  *
  * Layouts.  A tensor is `rows` x `cols` elements with a row stride given in ELEMENTS.
  *   separate gate/up  : in_row_stride == out_row_stride == cols
@@ -353,7 +354,11 @@ SWIGLU_B200_API int swiglu_b200_ckpt8_bwd(void* h, void* dgate, void* dup, const
  *   x        m x k, row stride x_row_stride; 16-byte aligned rows (a stride that is a multiple of 8 when m > 1)
  *   y, h     m x n, row stride given; may not overlap x or the weights
  *   group    32, 64 or 128 columns share a scale
- * Meant for m up to a few tens: every 32 tokens read the weights again. */
+ * Meant for m up to a few tens: every 32 tokens read the weights again.  One or two tokens are multiplied as 23-bit
+ * integers relative to the largest magnitude of their 256 columns (a token with an Inf or a NaN gives NaN); more go
+ * through 16-bit products.  The order of every sum is fixed.
+ * A call's kernel may start while the kernel of the linear / gate_up call before it on the stream is finishing; it reads
+ * and writes nothing of the caller's until everything enqueued earlier is complete. */
 SWIGLU_B200_API int swiglu_b200_w4_linear(void* y, const void* x, const void* blocks, int zeros, int64_t m, int64_t n,
                           int64_t k, int64_t x_row_stride, int64_t y_row_stride, int group, int dtype, int device,
                           void* stream);
