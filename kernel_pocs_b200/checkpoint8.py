@@ -50,8 +50,9 @@ class Checkpoint8:
 
     def __init__(self, data, shape, dtype, activation="silu", gate_multiplier=1.0, down_multiplier=1.0):
         shape = torch.Size(shape)
-        if data.dtype != torch.uint8 or data.dim() != 1 or data.numel() != Checkpoint8.size(shape):
-            raise ValueError(f"the kept form of shape {tuple(shape)} is {Checkpoint8.size(shape)} bytes")
+        if (data.dtype != torch.uint8 or data.dim() != 1 or data.numel() != Checkpoint8.size(shape)
+                or not data.is_contiguous()):
+            raise ValueError(f"the kept form of shape {tuple(shape)} is {Checkpoint8.size(shape)} bytes in a row")
         self.data = data
         self.shape = shape
         self.dtype = dtype
@@ -222,7 +223,7 @@ def _gradients(dout, kept: Checkpoint8, dgate: int, dup: int, grad_pitch: int, h
 def _check_dout(dout: torch.Tensor, kept: Checkpoint8) -> None:
     if dout.dtype != kept.dtype or dout.device != kept.device:
         raise TypeError("dout must have the dtype and device of gate and up")
-    if dout.shape != kept.shape:
+    if dout.shape != kept.shape or kept.data.numel() != Checkpoint8.size(kept.shape):
         raise ValueError(f"dout of shape {tuple(dout.shape)} does not match gate of shape {tuple(kept.shape)}")
     _require_cuda(dout, "dout")
 
@@ -270,6 +271,7 @@ class ForgePackedCkpt8Function(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, gate_up, activation="silu", gate_multiplier=1.0, down_multiplier=1.0):
+        _check_packed_input(gate_up)
         n_cols = gate_up.shape[-1] // 2
         # the two halves of one tensor share a row pitch: nothing is copied unless gate_up itself is not in rows
         packed = gate_up if _row_view(gate_up) is not None else gate_up.contiguous()

@@ -37,6 +37,8 @@ _DTYPE_CODE = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16:
 # ------------------------------------------------------------------------------------------
 
 def _as_float(name: str, value) -> float:
+    if type(value) is float:
+        return value
     if isinstance(value, torch.Tensor):
         raise TypeError(f"{name} must be a Python scalar, not a tensor")
     if not isinstance(value, numbers.Real):

@@ -62,7 +62,7 @@ class W4Weight:
     The constructor lays them out once in ``blocks``, the form the kernels read (``swiglu_b200_w4_linear`` in the C
     header), and keeps only that; ``packed``, ``scales`` and ``zeros`` are rebuilt on request."""
 
-    __slots__ = ("blocks", "dtype", "out_features", "in_features", "group_size", "has_zeros", "_operand")
+    __slots__ = ("_blocks", "dtype", "out_features", "in_features", "group_size", "has_zeros")
 
     def __init__(self, packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, *,
                  in_features: int, group_size: int = 128):
@@ -97,11 +97,16 @@ class W4Weight:
         parts = [p.permute(0, 3, 1, 2, 5, 4, 6).reshape(rows, cols, -1), self._tile_groups(scales)]
         if zeros is not None:
             parts.append(self._tile_groups(zeros))
-        self._set_blocks(torch.cat(parts, dim=2))
+        self._blocks = torch.cat(parts, dim=2)
 
-    def _set_blocks(self, blocks: torch.Tensor) -> None:
-        self.blocks = blocks  # uint8 [row tiles, column tiles, bytes of a block]
-        self._operand = (blocks.data_ptr(), int(self.has_zeros))
+    @property
+    def blocks(self) -> torch.Tensor:
+        """uint8 ``[row tiles, column tiles, bytes of a block]``."""
+        return self._blocks
+
+    def _operand(self):
+        # the address is asked for at every call: a copy of this object has blocks of its own
+        return self._blocks.data_ptr(), self.has_zeros
 
     def _tiles(self):
         return _ceil(self.out_features, TILE_ROWS), _ceil(self.in_features, TILE_COLS)
@@ -115,14 +120,14 @@ class W4Weight:
 
     def _untile_groups(self, lo: int, dtype: torch.dtype) -> torch.Tensor:
         (rows, cols), per = self._tiles(), TILE_COLS // self.group_size
-        t = self.blocks[:, :, lo:lo + 16 * per * dtype.itemsize].contiguous().view(dtype)
+        t = self._blocks[:, :, lo:lo + 16 * per * dtype.itemsize].contiguous().view(dtype)
         t = t.view(rows, cols, 8, per, 2).permute(0, 4, 2, 1, 3).reshape(TILE_ROWS * rows, cols * per)
         return t[:self.out_features, :_ceil(self.in_features, self.group_size)].contiguous()
 
     @property
     def packed(self) -> torch.Tensor:
         rows, cols = self._tiles()
-        p = self.blocks[:, :, :CODE_BYTES].reshape(rows, cols, 2, 8, 4, 4, 4).permute(0, 2, 3, 1, 5, 4, 6)
+        p = self._blocks[:, :, :CODE_BYTES].reshape(rows, cols, 2, 8, 4, 4, 4).permute(0, 2, 3, 1, 5, 4, 6)
         p = _shuffle(p, _FROM_BLOCK).reshape(TILE_ROWS * rows, 64 * cols)
         return p[:self.out_features, :16 * _ceil(self.in_features, 32)].contiguous()
 
@@ -142,33 +147,33 @@ class W4Weight:
 
     @property
     def device(self) -> torch.device:
-        return self.blocks.device
+        return self._blocks.device
 
     @property
     def nbytes(self) -> int:
         """Bytes the kernels read of it."""
-        return self.blocks.numel()
+        return self._blocks.numel()
 
     def to(self, device) -> "W4Weight":
         """This weight on ``device`` (itself when it is there already)."""
-        moved = self.blocks.to(device)
-        if moved is self.blocks:
+        moved = self._blocks.to(device)
+        if moved is self._blocks:
             return self
         other = object.__new__(W4Weight)
         for name in ("dtype", "out_features", "in_features", "group_size", "has_zeros"):
             setattr(other, name, getattr(self, name))
-        other._set_blocks(moved)
+        other._blocks = moved
         return other
 
     def dequantize(self) -> torch.Tensor:
         """``[out_features, in_features]`` in the dtype of the scales: ``(code - zero) * scale`` rounded once."""
-        if not self.blocks.is_cuda:
+        if not self._blocks.is_cuda:
             raise RuntimeError("W4Weight.dequantize has a CUDA (sm_100a) kernel only; there is no CPU fallback")
         n, k = self.shape
         out = torch.empty((n, k), dtype=self.dtype, device=self.device)
         _lib.check(
             "W4Weight.dequantize",
-            _lib.lib.swiglu_b200_w4_dequantize(out.data_ptr(), *self._operand, n, k, k, self.group_size,
+            _lib.lib.swiglu_b200_w4_dequantize(out.data_ptr(), *self._operand(), n, k, k, self.group_size,
                                                _DTYPE_CODE[self.dtype], self.device.index, _stream(self.device)),
         )
         return out
@@ -219,7 +224,7 @@ def quantize_w4(weight: torch.Tensor, group_size: int = 128, zero_points: bool =
 
 
 def _check_tokens(x: torch.Tensor, w: W4Weight, what: str) -> None:
-    if not (x.is_cuda and w.blocks.is_cuda):
+    if not (x.is_cuda and w._blocks.is_cuda):
         raise RuntimeError(f"{what} has a CUDA (sm_100a) kernel only; there is no CPU fallback")
     if x.device != w.device:
         raise ValueError(f"x is on {x.device}, the weight on {w.device}")
@@ -256,7 +261,7 @@ def w4_linear(x: torch.Tensor, weight: W4Weight) -> torch.Tensor:
     device = x.device
     _lib.check(
         "w4_linear",
-        _lib.lib.swiglu_b200_w4_linear(y.data_ptr(), x.data_ptr(), *weight._operand, m, n, k, pitch, n,
+        _lib.lib.swiglu_b200_w4_linear(y.data_ptr(), x.data_ptr(), *weight._operand(), m, n, k, pitch, n,
                                        weight.group_size, _DTYPE_CODE[x.dtype], device.index, _stream(device)),
     )
     return y
@@ -286,11 +291,11 @@ def w4_gate_up(x: torch.Tensor, w_gate: W4Weight, w_up: W4Weight, activation: st
     on the way."""
     _check_activation(activation)
     gm, dm = _check_multipliers(activation, gate_multiplier, down_multiplier)
-    if (w_gate.out_features != w_up.out_features or w_gate.in_features != w_up.in_features
-            or w_gate.group_size != w_up.group_size or w_gate.dtype != w_up.dtype or w_gate.device != w_up.device):
+    n, k = w_gate.out_features, w_gate.in_features
+    if (n != w_up.out_features or k != w_up.in_features or w_gate.group_size != w_up.group_size
+            or w_gate.dtype != w_up.dtype or w_gate.device != w_up.device):
         raise ValueError("w_gate and w_up must agree in shape, group size, dtype and device")
     _check_tokens(x, w_gate, "w4_gate_up")
-    n, k = w_gate.out_features, w_gate.in_features
     m = x.numel() // k
     if m > GATE_UP_ROWS:
         return _gate_up_16bit(x, w_gate, w_up, activation, gm, dm)
@@ -300,7 +305,7 @@ def w4_gate_up(x: torch.Tensor, w_gate: W4Weight, w_up: W4Weight, activation: st
     _lib.check(
         "w4_gate_up",
         _lib.lib.swiglu_b200_w4_gate_up(
-            h.data_ptr(), x.data_ptr(), *w_gate._operand, *w_up._operand, m, n, k, pitch, n, w_gate.group_size,
+            h.data_ptr(), x.data_ptr(), *w_gate._operand(), *w_up._operand(), m, n, k, pitch, n, w_gate.group_size,
             _DTYPE_CODE[x.dtype], ACTIVATIONS[activation], gm, dm, device.index, _stream(device),
         ),
     )

@@ -119,8 +119,12 @@ def test_refusals():
     kept = Checkpoint8(torch.ones(Checkpoint8.size((4, 8)), dtype=torch.uint8), (4, 8), torch.float32)
     with pytest.raises(ValueError, match="is 264 bytes"):
         Checkpoint8(torch.ones(263, dtype=torch.uint8), (4, 8), torch.float32)
+    with pytest.raises(ValueError, match="in a row"):
+        Checkpoint8(torch.ones(528, dtype=torch.uint8)[::2], (4, 8), torch.float32)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         ckpt8_backward(torch.zeros(4, 8), kept)
+    with pytest.raises(ValueError, match="must be even"):
+        checkpoint8.ForgePackedCkpt8Function.apply(torch.zeros(4, 7))
     with pytest.raises(ValueError, match="does not match"):
         ckpt8_backward(torch.zeros(4, 9), kept)
     with pytest.raises(TypeError, match="dtype and device"):

@@ -130,6 +130,18 @@ def test_quantiser_is_within_half_a_step(dtype, n, k, group, zero_points):
     assert not bool(got[0].any())
 
 
+def test_copies_have_blocks_of_their_own():
+    import copy
+    import pickle
+
+    w = W4Weight(*random_parts(20, 200, 64, True, torch.float16), in_features=200, group_size=64)
+    for other in (copy.deepcopy(w), pickle.loads(pickle.dumps(w))):
+        assert torch.equal(other.blocks, w.blocks) and other.shape == w.shape and other.dtype == w.dtype
+        assert other._operand()[0] == other.blocks.data_ptr() != w.blocks.data_ptr()
+    with pytest.raises(AttributeError):
+        w.blocks = w.blocks[:1]
+
+
 def test_refusals():
     packed, scales, z = random_parts(4, 64, 32, True, torch.bfloat16)
     ok = dict(in_features=64, group_size=32)
@@ -285,14 +297,14 @@ def test_pitched_and_misaligned_tokens(dtype, m, offset, extra):
     out = torch.full((16 + m * (n + 5),), 55.0, dtype=dtype, device="cuda")
     y = out[8:8 + m * (n + 5)].view(m, n + 5)[:, :n]
     st = torch.cuda.current_stream().cuda_stream
-    assert _lib.lib.swiglu_b200_w4_linear(y.data_ptr(), x.data_ptr(), *w._operand, m, n, k, k, n + 5, 64,
+    assert _lib.lib.swiglu_b200_w4_linear(y.data_ptr(), x.data_ptr(), *w._operand(), m, n, k, k, n + 5, 64,
                                           CODES[dtype], -1, st) == 0
     assert torch.equal(y, want)
     y.fill_(55.0)
     assert bool((out == 55.0).all())
     full = torch.full((n * (k + 7) + 16,), 55.0, dtype=dtype, device="cuda")
     d = full[5:5 + n * (k + 7)].view(n, k + 7)[:, :k]
-    assert _lib.lib.swiglu_b200_w4_dequantize(d.data_ptr(), *w._operand, n, k, k + 7, 64, CODES[dtype], -1, st) == 0
+    assert _lib.lib.swiglu_b200_w4_dequantize(d.data_ptr(), *w._operand(), n, k, k + 7, 64, CODES[dtype], -1, st) == 0
     assert torch.equal(d, w.dequantize())
     d.fill_(55.0)
     assert bool((full == 55.0).all())
