@@ -4,12 +4,12 @@
 //   h[m][n] = act(gm * (x . w_gate[n])) * (x . w_up[n]) * dm               both projections in one launch
 //
 // With a handful of tokens the weights' bytes are the whole cost (n*k/2, each used 2m times), so the kernels are
-// streams of weights with as little arithmetic per weight as it takes.  The products go through mma.sync m16n8k16: 16
-// weight rows are the A operand, 8 tokens the B operand, accumulation in fp32.  The tensor pipe is far from busy here;
-// what the instruction saves is issue slots (one weight per lane and FMA would need 8 m of them for 8 weights).  Eight
-// nibbles become four pairs of 16-bit numbers with a mask, an OR that puts them into the mantissa of 128 (bf16) or 1024
-// (fp16), and an exact subtraction of that plus the zero point.  q - z is exact in either type; the sum over a group is
-// a fp32 accumulator which is multiplied by the group's scale in fp32: nothing is rounded to 16 bits before the result.
+// streams of weights with as little arithmetic per weight as it takes: 8-bit integer products for one or two tokens,
+// mma.sync m16n8k16 for a few with few weights, tcgen05 for the rest.  The tensor pipes are far from busy in all of them;
+// what the instructions save is issue slots (one weight per lane and FMA would need 8 m of them for 8 weights).  For the
+// 16-bit products eight nibbles become four pairs of numbers q - z, exact in either type, with a mask and a multiply-add
+// for each.  The sum over a group is an accumulator of 32 bits which is multiplied by the group's scale in fp32: nothing is
+// rounded to 16 bits before the result.
 //
 // Weight blocks.  The fragments fix which lane needs which nibbles, so weights are laid out once for it: 16 rows x 128
 // columns are 1 KB in which lane l = 4g + t finds the 32 nibbles of row g (and, 512 bytes on, of row g + 8) that it
@@ -24,6 +24,7 @@
 
 #include "launch_common.cuh"
 #include "swiglu_kernels.cuh"
+#include "tcgen05_common.cuh"
 
 namespace {
 
@@ -49,6 +50,7 @@ struct W4Shape {
   int col_tiles;
   int groups_log2;  // log2 of the groups per column tile (0, 1, 2)
   int split;        // CTAs that share a row of column tiles, a cluster
+  int row_groups;   // of a cluster (w4_mma_kernel)
   int share, over;  // column tiles (or pairs) of each, and how many of them take one more
   int slice;        // outputs that each finishes
   int y_vec;        // groups of 4 outputs can be stored as one
@@ -156,6 +158,7 @@ __device__ __forceinline__ uint32_t cluster_index() {
   return r;
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 // Stores v at `addr` of the shared memory of CTA `rank` of the cluster.
 __device__ __forceinline__ void cluster_store(uint32_t addr, uint32_t rank, float v) {
@@ -179,9 +182,26 @@ __device__ __forceinline__ float result(const float (&v)[MATS], int activation, 
   else return Math<true, ACT_GELU_ERF>::fwd(v[0], v[1], c);
 }
 
+// Stores the results of rows n .. n+3, as far as they exist, of the token whose outputs start at `row`.
+template <class T, int MATS>
+__device__ __forceinline__ void store_results(void* y, long long row, long long n, const W4Shape& s, const float (&v)[4][MATS],
+                                              int activation, const Consts& c) {
+  uint16_t out[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = Half2<T>::from_float(result<MATS>(v[i], activation, c));
+  uint16_t* to = static_cast<uint16_t*>(y) + row + n;
+  if (s.y_vec && n + 4 <= s.n) {
+    *reinterpret_cast<uint2*>(to) = make_uint2(out[0] | (uint32_t)out[1] << 16, out[2] | (uint32_t)out[3] << 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < s.n) to[i] = out[i];
+  }
+}
+
 constexpr int kTokenBytes = kTileCols * 2;  // a token's part of a column tile
 
-// ------------------------------------------------------------------ up to 32 tokens: 16-bit products
+// ------------------------------------------------------------------ up to 32 tokens, few weights: mma.sync
 
 // Shared memory of a CTA: DEPTH stages of one column tile each, then where the cluster's sums arrive.
 template <int MATS, int NT, int GROUPS> struct Cfg {
@@ -198,8 +218,8 @@ template <int MATS, int NT, int GROUPS> struct Cfg {
 };
 
 // A CTA owns 8 row tiles (one to a warp; two would read the tokens' fragments once for both, but 128 rows to a CTA
-// balance better: fp16 32 x 5504 -> 11009 21.6 us against 23.5) of MATS matrices, 8 * NT tokens and, as rank r of a cluster of `split`
-// CTAs, the r-th part of the column tiles.  Each rank finishes a slice of the outputs: the others store their sums for
+// balance better: fp16 32 x 5504 -> 11009 21.6 us against 23.5) of MATS matrices, 8 * NT tokens and, as rank r of a
+// cluster of `split` CTAs, the r-th part of the column tiles.  Each rank finishes a slice of the outputs: the others store their sums for
 // it into its shared memory, where they are added in a fixed order.
 template <class T, int MATS, int NT, int GROUPS>
 __global__ void __launch_bounds__(32 * kWarps, Cfg<MATS, NT, GROUPS>::CTAS)
@@ -389,17 +409,298 @@ w4_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, int acti
       }
       v[0][a] = f.x, v[1][a] = f.y, v[2][a] = f.z, v[3][a] = f.w;
     }
-    uint16_t out[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) out[i] = H::from_float(result<MATS>(v[i], activation, consts));
-    uint16_t* to = static_cast<uint16_t*>(y) + (token0 + tok) * s.y_pitch + n;
-    if (s.y_vec && n + 4 <= s.n) {
-      *reinterpret_cast<uint2*>(to) = make_uint2(out[0] | (uint32_t)out[1] << 16, out[2] | (uint32_t)out[3] << 16);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n + i < s.n) to[i] = out[i];
+    store_results<T, MATS>(y, (token0 + tok) * s.y_pitch, n, s, v, activation, consts);
+  }
+}
+
+// ------------------------------------------------------------------ more tokens or weights: tcgen05
+//
+// 128 rows of weights are the M of tcgen05.mma, 16, 32 or 64 tokens its N.  A thread keeps one row: it reads the 64 bytes
+// of codes that the row has in a block, turns them into pairs of 16-bit numbers as above and stores them as A in its lane
+// of the tensor memory, from where the tensor core reads them; the tokens are B, which it reads from shared memory as a
+// tiled copy has laid them out.  Against mma.sync no warp reads tokens any more (with 32 of them that was 64 of the 82
+// accesses to shared memory for a block), and the work for a weight is the same for any number of tokens.  The products
+// of a scale group are read back, and scaled and added up in registers.
+//
+// A kernel that allocates tensor memory runs with one CTA to an SM, so a CTA has four such warpgroups, which work on
+// column tiles of their own.  While one waits for its products the others turn codes into numbers; what bounds the kernel
+// are the instructions for that (bf16 32 x 4096 -> 14336 gate and up: 84 % of the issue slots of the busy SMs).
+
+constexpr int kGroupThreads = 128, kGroups = 4;  // warpgroups, a thread to a weight row
+constexpr int kGroupRows = 128;
+
+// Distance of the blocks of a column tile in shared memory: an odd multiple of 16, so that four of them start in different
+// banks.  The copies bring what follows a block along.
+__host__ __device__ constexpr int slot_bytes(int groups, bool zeros) { return block_bytes(groups, zeros) | 16; }
+
+// What w4_mma_kernel copies from: the tokens, and each matrix as [row tiles][bytes] in elements of 8 bytes.
+struct Maps {
+  CUtensorMap x, w[2];
+};
+
+// Shared memory of a CTA: DEPTH stages of each warpgroup's column tile of the tokens, then of its blocks; where the
+// cluster's sums arrive takes the place of the stages.
+template <int N, int GROUPS> struct MmaCfg {
+  static constexpr int SLOT = slot_bytes(GROUPS, true);
+  static constexpr int X = N * kTokenBytes, TILES = kGroupRows / kTileRows;
+  // swizzled tiles start on multiples of 1024
+  static constexpr int STAGE = (kGroups * (X + TILES * SLOT) + 1023) / 1024 * 1024;
+  static constexpr int FIT = 224 * 1024 / STAGE, DEPTH = FIT > 6 ? 6 : FIT;
+  static constexpr int SMEM = 1024 + DEPTH * STAGE;  // the first kilobyte is lost to alignment
+  static constexpr int A_COLS = kTileCols / 2, D_COLS = 64, TMEM = kGroups * (A_COLS + D_COLS);
+  static constexpr int AT_ONCE = D_COLS / N < GROUPS ? D_COLS / N : GROUPS;  // groups whose products are held at a time
+  // the cluster's sums take the place of the stages: those that arrive, and as many tokens of those that leave as fit
+  static constexpr int ARRIVALS = (kGroups * N + 32) * kGroupRows * 4, LEAVING = N < 64 ? N : 16;
+  static_assert(DEPTH >= 2 && ARRIVALS + kGroups * LEAVING * kGroupRows * 4 <= DEPTH * STAGE, "room for the sums");
+};
+
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// D (+)= A B with A in tensor memory
+__device__ __forceinline__ void mma_from_tmem(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a),
+      "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tile_load(uint32_t dst, const CUtensorMap& map, int col, int row, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(&map), "r"(col), "r"(row), "r"(tc::smem_u32(bar))
+      : "memory");
+}
+// Waits for a barrier that only this CTA's own copies or products arrive at; false after half a second.
+__device__ __forceinline__ bool own_wait(uint64_t* bar, uint32_t parity) {
+  if (tc::mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!tc::mbar_try_wait(bar, parity))
+    if (clock64() - t0 > tc::WAIT_CYCLES) return false;
+  return true;
+}
+// True for one lane of a warp whose lanes all take part.
+__device__ __forceinline__ bool elect() {
+  uint32_t one;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(one));
+  return one != 0;
+}
+__device__ __forceinline__ void group_sync(int group) {  // of a warpgroup
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(kGroupThreads) : "memory");
+}
+
+// A cluster of `split` CTAs owns `row_groups` times 128 rows of MATS matrices and N tokens.
+template <class T, int MATS, int N, int GROUPS>
+__global__ void __launch_bounds__(kGroups * kGroupThreads, 1)
+w4_mma_kernel(void* y, const __grid_constant__ Maps maps, W4 w0, W4 w1, W4Shape s, int activation, float gm, float dm) {
+  using H = Half2<T>;
+  using C = MmaCfg<N, GROUPS>;
+  constexpr int DEPTH = C::DEPTH, TILES = C::TILES;
+  extern __shared__ unsigned char raw_smem[];
+  __shared__ uint32_t tmem_slot;
+  __shared__ __align__(8) uint64_t products[kGroups], full[kGroups][DEPTH];
+  let_next_start();
+  const uint32_t smem_addr = ((uint32_t)__cvta_generic_to_shared(raw_smem) + 1023u) & ~1023u;
+  unsigned char* smem = raw_smem + (smem_addr - (uint32_t)__cvta_generic_to_shared(raw_smem));
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, quarter = warp & 3;
+  const int group = warp >> 2;  // the warpgroup
+  // A thread's lane of the tensor memory, and the row of the weights that it holds.  Any order of the rows will do; in
+  // this one the eight threads that read together touch two rows of each of four blocks, which are in different banks.
+  const int tile = (quarter >> 1) * 4 + (lane & 3), in_tile = (quarter & 1) * 8 + (lane >> 2), row = tile * kTileRows + in_tile;
+  // The cluster's row groups and matrices are dealt to its warpgroups, `parts` of them to each, which share its column tiles.
+  const int rank = (int)cluster_rank(), worker = rank * kGroups + group, jobs = s.row_groups * MATS;
+  const int part = worker / jobs, parts = s.split * kGroups / jobs, job = worker - part * jobs;
+  const int matrix = job % MATS, row_group = job / MATS;  // the latter in the cluster
+  const int row_tiles = (int)((s.n + kTileRows - 1) / kTileRows);
+  const int row_tile0 = ((int)cluster_index() * s.row_groups + row_group) * TILES;
+  const int tiles = max(0, min(TILES, row_tiles - row_tile0));
+  const int token0 = (int)blockIdx.y * N;
+  const W4 w = matrix ? w1 : w0;
+  const int bytes = block_bytes(GROUPS, w.zeros);
+  const int share = s.col_tiles / parts, over = s.col_tiles % parts;
+  const int first = part * share + min(part, over), last = tiles > 0 ? first + share + (part < over ? 1 : 0) : first;
+  const int tokens = s.m - token0 < N ? (int)(s.m - token0) : N;
+
+  const uint32_t w_at = kGroups * C::X + group * TILES * C::SLOT;  // in a stage
+  const int slot = slot_bytes(GROUPS, w.zeros);
+  int fill = 0;  // the stage to fill next
+  // Starts the copies of column tile c, from one thread of the warpgroup's second warp: an instruction takes about a hundred
+  // cycles to leave, and this warp has nothing to do while the first one starts the products.
+  auto fetch = [&](int c) {
+    if (elect()) {
+      uint64_t* bar = &full[group][fill];
+      const uint32_t to = smem_addr + fill * C::STAGE;
+      tc::mbar_expect_tx(bar, C::X + TILES * slot);
+      tile_load(to + w_at, maps.w[matrix], c * (bytes / 8), row_tile0, bar);
+      tile_load(to + group * C::X, maps.x, c * kTileCols, token0, bar);
+      tile_load(to + group * C::X + N * 128, maps.x, c * kTileCols + 64, token0, bar);
     }
+    fill = fill == DEPTH - 1 ? 0 : fill + 1;
+  };
+
+  if (threadIdx.x % kGroupThreads < tiles && first < last)
+    prefetch_l2(cbyte(w.blocks) + ((long long)(row_tile0 + (int)threadIdx.x % kGroupThreads) * s.col_tiles + first) * bytes,
+                min(DEPTH, last - first) * bytes);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kGroups; ++i) {
+      tc::mbar_init(&products[i], 1);
+      for (int d = 0; d < DEPTH; ++d) tc::mbar_init(&full[i][d], 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  __syncthreads();
+  wait_for_previous();
+  if (quarter == 1 && first < last) fetch(first);
+  __syncwarp();
+  // Only now: a launch that waits for the one before it must not hold tensor memory which that one still asks for.  It
+  // is given back before the CTA waits for any other.
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&tmem_slot)),
+                 "n"(C::TMEM) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0) + group * (C::A_COLS + C::D_COLS);
+  const uint32_t tmem_row = tmem + ((uint32_t)(quarter * 32) << 16);
+  constexpr uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  constexpr uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | ((N >> 3) << 17) | ((128u >> 4) << 24);
+
+  if (quarter == 1) {
+#pragma unroll 1
+    for (int i = 1; i < DEPTH && first + i < last; ++i) fetch(first + i);
+  }
+  float acc[N] = {};
+  bool ok = true;
+  uint32_t parity = 0;
+  int take = 0, round = 0;  // the stage to read next, and how often it has been filled before, modulo 2
+#pragma unroll 1
+  for (int c = first; c < last; ++c) {
+    ok = ok && own_wait(&full[group][take], round);
+    const unsigned char* block = smem + w_at + take * C::STAGE + tile * slot;
+    const unsigned char* tail = block + kTileBytes;
+    const int at = (in_tile & 7) * GROUPS * 2 + (in_tile >> 3);  // of the first group's scale
+    uint4 codes[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) codes[t] = *reinterpret_cast<const uint4*>(block + in_tile * 64 + t * 16);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      constexpr int per_group = 4 / GROUPS;  // words per group
+      uint32_t bias = H::pair(-8.0f * H::kUnit);
+      if (w.zeros) bias = H::pair(-H::kUnit * zero_point(tail[GROUPS * 32 + at + u / per_group * 2]));
+      uint32_t a[16];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const uint32_t words[4] = {codes[t].x, codes[t].y, codes[t].z, codes[t].w};
+        uint32_t p[4];
+        weight_pairs<T>(words[u], bias, p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[4 * t + i] = p[i];
+      }
+      tmem_st16(tmem_row + 16 * u, a);
+    }
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int g0 = 0; g0 < GROUPS; g0 += C::AT_ONCE) {
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      group_sync(group);  // all of A and of the tokens is there, what D held has been read
+      if (quarter == 0) {
+        if (elect()) {
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint64_t b = tc::umma_desc(smem_addr + group * C::X + take * C::STAGE);
+#pragma unroll
+          for (int g = 0; g < C::AT_ONCE; ++g)
+#pragma unroll
+            for (int i = 0; i < 8 / GROUPS; ++i) {  // 16 columns each
+              const int kk = (g0 + g) * (8 / GROUPS) + i;
+              mma_from_tmem(tmem + C::A_COLS + g * N, tmem + 8 * kk, b + (kk >> 2) * (N * 128 / 16) + 2 * (kk & 3), idesc,
+                            i != 0);
+            }
+          tc::umma_commit(&products[group]);
+        }
+      } else if (quarter == 1 && g0 == 0 && c > first && c - 1 + DEPTH < last) {
+        fetch(c - 1 + DEPTH);  // the stage before this one has been read by all
+      }
+      __syncwarp();
+      ok = ok && own_wait(&products[group], parity);
+      parity ^= 1;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+      for (int g = 0; g < C::AT_ONCE; ++g) {
+        const float scale = H::to_float(*reinterpret_cast<const uint16_t*>(tail + (at + (g0 + g) * 2) * 2));
+        constexpr int STEP = N < 32 ? 16 : 32;
+#pragma unroll
+        for (int j0 = 0; j0 < N; j0 += STEP) {
+          uint32_t d[STEP];
+          if constexpr (STEP == 16) tc::tmem_ld16(tmem_row + C::A_COLS + g * N + j0, d);
+          else tc::tmem_ld32(tmem_row + C::A_COLS + g * N + j0, d);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int j = 0; j < STEP; ++j) acc[j0 + j] = fmaf(__uint_as_float(d[j]), scale, acc[j0 + j]);
+        }
+      }
+    }
+    if (++take == DEPTH) {
+      take = 0;
+      round ^= 1;
+    }
+  }
+
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  const bool failed = __syncthreads_or(!ok);
+  if (failed) {  // copies and products may still be under way
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000LL) {
+    }
+  }
+  cluster_arrive_relaxed();  // nothing was written for the others yet
+  if (warp == 0) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_slot), "n"(C::TMEM) : "memory");
+  }
+  cluster_wait();  // no CTA of the cluster needs its stages any more
+  // Each rank finishes `slice` of the cluster's [row group][token].  What arrives there: [matrix][part][of the slice][row].
+  const int slice = s.slice;
+  const int mine = min(slice, s.row_groups * tokens - rank * slice);
+  const float unit = failed ? __uint_as_float(0x7fffffffu) : 1.0f / H::kUnit;
+  const uint32_t to = smem_addr + (matrix * parts + part) * slice * (kGroupRows * 4) + lane * 16;
+  unsigned char* leaving = smem + C::ARRIVALS + group * (C::LEAVING * kGroupRows * 4);  // [token][row] of this warpgroup
+#pragma unroll
+  for (int j0 = 0; j0 < N; j0 += C::LEAVING) {
+    if (j0 != 0) group_sync(group);
+#pragma unroll
+    for (int j = 0; j < C::LEAVING; ++j) *reinterpret_cast<float*>(leaving + (j * kGroupRows + row) * 4) = acc[j0 + j] * unit;
+    group_sync(group);
+#pragma unroll 1
+    for (int j = quarter; j < C::LEAVING && j0 + j < tokens; j += 4) {  // a warp to a token
+      const int i = row_group * tokens + j0 + j, owner = i / slice;
+      cluster_store4(to + (i - owner * slice) * (kGroupRows * 4), owner,
+                     *reinterpret_cast<const float4*>(leaving + j * (kGroupRows * 4) + lane * 16));
+    }
+  }
+  cluster_arrive();
+  cluster_wait();
+  const Consts consts(gm, dm);
+#pragma unroll 1
+  for (int o = warp; o < mine; o += kGroups * 4) {  // a warp to a token, a lane to four rows
+    const int unit_row = (rank * slice + o) / tokens, token = (rank * slice + o) - unit_row * tokens;
+    const long long n = ((long long)cluster_index() * s.row_groups + unit_row) * kGroupRows + 4 * lane;
+    if (n >= s.n) continue;
+    float v[4][MATS] = {};
+#pragma unroll 1
+    for (int i = 0; i < parts; ++i)
+#pragma unroll
+      for (int a = 0; a < MATS; ++a) {
+        const float4 f =
+            *reinterpret_cast<const float4*>(smem + ((a * parts + i) * slice + o) * (kGroupRows * 4) + lane * 16);
+        v[0][a] += f.x, v[1][a] += f.y, v[2][a] += f.z, v[3][a] += f.w;
+      }
+    store_results<T, MATS>(y, ((long long)token0 + token) * s.y_pitch, n, s, v, activation, consts);
   }
 }
 
@@ -772,7 +1073,7 @@ int launched() {
   return SWIGLU_B200_OK;
 }
 
-constexpr long long kMaxSize = 1LL << 31;  // of n and k: tile counts fit an int, byte offsets 62 bits
+constexpr long long kMaxSize = 1LL << 30;  // of n and k: tile counts and copies' coordinates fit an int, byte offsets 62 bits
 
 // Checks shared by the three entries; fills the shape.
 int check(const W4* w, int mats, int64_t n, int64_t k, int group, int dtype, W4Shape& s) {
@@ -807,60 +1108,86 @@ struct Launcher {
   std::atomic<int> clusters[64][9] = {};
 };
 
+template <class X> using Kernel = void (*)(void*, X, W4, W4, W4Shape, int, float, float);
+
+// One of the kernels above on the current device.
+template <class X> struct Start {
+  Kernel<X> kernel;
+  Launcher& known;
+  int threads, smem, device = 0;
+  cudaLaunchAttribute attrs[2] = {};
+  cudaLaunchConfig_t cfg{};
+
+  Start(Kernel<X> kernel, Launcher& known, int threads, int smem)
+      : kernel(kernel), known(known), threads(threads), smem(smem) {}
+
+  int prepare(cudaStream_t st) {
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess && !(device < 64 && (known.opted_in.load(std::memory_order_relaxed) >> device & 1))) {
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (e == cudaSuccess && device < 64) known.opted_in.fetch_or(1ULL << device, std::memory_order_relaxed);
+    }
+    if (e != cudaSuccess) return note_cuda_error(SWIGLU_B200_ERR_DEVICE, e);
+    attrs[0].id = cudaLaunchAttributeClusterDimension;
+    attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
+    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cfg.attrs = attrs;
+    return SWIGLU_B200_OK;
+  }
+  // How many clusters of `split` CTAs run at once; negative: an error code.
+  int at_once(int split) {
+    int n = device < 64 ? known.clusters[device][split].load(std::memory_order_relaxed) : 0;
+    if (n == 0) {
+      attrs[0].val.clusterDim.x = (unsigned)split;
+      cfg.gridDim = dim3((unsigned)split);
+      cfg.numAttrs = 1;
+      const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+      if (e != cudaSuccess) return -note_cuda_error(SWIGLU_B200_ERR_DEVICE, e);
+      if (device < 64) known.clusters[device][split].store(n, std::memory_order_relaxed);
+    }
+    return n;
+  }
+  int launch(long long clusters, long long gy, void* y, const X& x, const W4* w, int mats, const W4Shape& s, int activation,
+             float gm, float dm) {
+    attrs[0].val.clusterDim.x = (unsigned)s.split;
+    cfg.gridDim = dim3((unsigned)(clusters * s.split), (unsigned)gy);
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, y, x, w[0], w[mats - 1], s, activation, gm, dm);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return note_cuda_error(SWIGLU_B200_ERR_LAUNCH, e);
+    }
+    note_launch();
+    return SWIGLU_B200_OK;
+  }
+};
+
 // Launches `kernel` with one cluster for each of `clusters` x `gy`.  Its `parts` column tiles (or pairs) are split over
 // the CTAs of a cluster, as many as leave every cluster running at once: all of them stream from the start and end
 // together (one cluster more than fit is another round, 430 CTAs instead of 258 took 22.8 us instead of 19.9).
 // `outputs` are a cluster's, finished in slices of a multiple of `unit`.
-template <class... P>
-int start(void (*kernel)(P...), Launcher& known, long long clusters, long long gy, int parts, int outputs, int unit,
-          int smem, cudaStream_t st, void* y, const void* x, const W4& w0, const W4& w1, W4Shape s, int activation,
-          float gm, float dm) {
+int start(Kernel<const void*> kernel, Launcher& known, long long clusters, long long gy, int parts, int outputs, int unit,
+          int smem, cudaStream_t st, void* y, const void* x, const W4* w, int mats, W4Shape s, int activation, float gm,
+          float dm) {
   if (clusters > 0x7fffffffLL / 8 || gy > 65535) return SWIGLU_B200_ERR_SHAPE;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && !(dev < 64 && (known.opted_in.load(std::memory_order_relaxed) >> dev & 1))) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess && dev < 64) known.opted_in.fetch_or(1ULL << dev, std::memory_order_relaxed);
-  }
-  if (e != cudaSuccess) return note_cuda_error(SWIGLU_B200_ERR_DEVICE, e);
-  cudaLaunchAttribute attrs[2] = {};
-  cudaLaunchAttribute& cluster = attrs[0];
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-  attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attrs[1].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.blockDim = dim3(32 * kWarps);
-  cfg.dynamicSmemBytes = (size_t)smem;
-  cfg.stream = st;
-  cfg.attrs = attrs;
-  cfg.numAttrs = 1;
+  Start<const void*> k(kernel, known, 32 * kWarps, smem);
+  int rc = k.prepare(st);
+  if (rc != SWIGLU_B200_OK) return rc;
   int split = parts < 8 ? parts : 8;
   for (; split > 1; --split) {
-    int at_once = dev < 64 ? known.clusters[dev][split].load(std::memory_order_relaxed) : 0;
-    if (at_once == 0) {
-      cluster.val.clusterDim.x = (unsigned)split;
-      cfg.gridDim = dim3((unsigned)split);
-      e = cudaOccupancyMaxActiveClusters(&at_once, kernel, &cfg);
-      if (e != cudaSuccess) return note_cuda_error(SWIGLU_B200_ERR_DEVICE, e);
-      if (dev < 64) known.clusters[dev][split].store(at_once, std::memory_order_relaxed);
-    }
+    const int at_once = k.at_once(split);
+    if (at_once < 0) return -at_once;
     if (clusters * gy <= at_once) break;
   }
   s.split = split;
   s.share = parts / split;
   s.over = parts % split;
   s.slice = (outputs + unit * split - 1) / (unit * split) * unit;
-  cluster.val.clusterDim.x = (unsigned)split;
-  cfg.gridDim = dim3((unsigned)(clusters * split), (unsigned)gy);
-  cfg.numAttrs = 2;
-  e = cudaLaunchKernelEx(&cfg, kernel, y, x, w0, w1, s, activation, gm, dm);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return note_cuda_error(SWIGLU_B200_ERR_LAUNCH, e);
-  }
-  note_launch();
-  return SWIGLU_B200_OK;
+  return k.launch(clusters, gy, y, x, w, mats, s, activation, gm, dm);
 }
 
 template <class T, int MATS, int NT, int GROUPS>
@@ -868,8 +1195,53 @@ int launch(void* y, const void* x, const W4* w, const W4Shape& s, int activation
   constexpr int kRows = kWarps * kTileRows;
   static Launcher known;
   return start(w4_kernel<T, MATS, NT, GROUPS>, known, (s.n + kRows - 1) / kRows, (s.m + 8 * NT - 1) / (8 * NT),
-               s.col_tiles, kRows * (int)(s.m < 8 * NT ? s.m : 8 * NT), 4, Cfg<MATS, NT, GROUPS>::SMEM, st, y, x, w[0],
-               w[MATS - 1], s, activation, gm, dm);
+               s.col_tiles, kRows * (int)(s.m < 8 * NT ? s.m : 8 * NT), 4, Cfg<MATS, NT, GROUPS>::SMEM, st, y, x, w,
+               MATS, s, activation, gm, dm);
+}
+
+template <class T, int MATS, int N, int GROUPS>
+int launch_mma(void* y, const void* x, const W4* w, const W4Shape& s, int activation, float gm, float dm, cudaStream_t st) {
+  static Launcher known;
+  const tc::EncodeTiled encode = tc::encode_fn();
+  if (!encode) return SWIGLU_B200_ERR_DEVICE;
+  Maps maps;
+  const cuuint32_t steps[2] = {1, 1};
+  const cuuint64_t x_dims[2] = {(cuuint64_t)s.k, (cuuint64_t)s.m}, x_pitch[1] = {(cuuint64_t)s.x_pitch * 2};
+  const cuuint32_t x_box[2] = {64, N};
+  bool mapped = encode(&maps.x, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(x), x_dims, x_pitch, x_box, steps,
+                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  for (int a = 0; a < MATS && mapped; ++a) {
+    const cuuint64_t pitch[1] = {(cuuint64_t)s.col_tiles * block_bytes(GROUPS, w[a].zeros)};
+    const cuuint64_t dims[2] = {pitch[0] / 8, (cuuint64_t)((s.n + kTileRows - 1) / kTileRows)};
+    const cuuint32_t box[2] = {(cuuint32_t)slot_bytes(GROUPS, w[a].zeros) / 8, kGroupRows / kTileRows};
+    mapped = encode(&maps.w[a], CU_TENSOR_MAP_DATA_TYPE_INT64, 2, const_cast<void*>(w[a].blocks), dims, pitch, box, steps,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  }
+  if (!mapped) return SWIGLU_B200_ERR_DEVICE;
+  Start<Maps> k(w4_mma_kernel<T, MATS, N, GROUPS>, known, kGroups * kGroupThreads, MmaCfg<N, GROUPS>::SMEM);
+  int rc = k.prepare(st);
+  if (rc != SWIGLU_B200_OK) return rc;
+  const long long row_groups = (s.n + kGroupRows - 1) / kGroupRows, gy = (s.m + N - 1) / N;
+  if (row_groups > 0x7fffffffLL / 8 || gy > 65535) return SWIGLU_B200_ERR_SHAPE;
+  // The fewest column tiles to a warpgroup with every cluster running at once: gate and up of 4096 -> 11008 have 86 groups
+  // of 128 rows, two to each of 43 clusters of three CTAs are 11 tiles to a warpgroup, one to each of 86 CTAs 16.
+  int best = 0, split = 1, groups = 1;
+  for (int r = 1; r <= 4; ++r)
+    for (int c = 1; c <= 8; ++c) {
+      if (kGroups * c % (r * MATS)) continue;
+      const int parts = kGroups * c / (r * MATS), cost = (s.col_tiles + parts - 1) / parts;
+      if (best != 0 && cost >= best) continue;
+      const int at_once = k.at_once(c);
+      if (at_once < 0) return -at_once;
+      if ((row_groups + r - 1) / r * gy <= at_once) best = cost, split = c, groups = r;
+    }
+  W4Shape shape = s;
+  shape.split = split;
+  shape.row_groups = groups;
+  shape.slice = (groups * (int)(s.m < N ? s.m : N) + split - 1) / split;
+  return k.launch((row_groups + groups - 1) / groups, gy, y, maps, w, MATS, shape, activation, gm, dm);
 }
 
 template <class T, int MATS, int GROUPS>
@@ -879,8 +1251,8 @@ int launch_digits(void* y, const void* x, const W4* w, const W4Shape& s, int act
   static Launcher known;
   return start(w4_digits_kernel<T, MATS, GROUPS>, known, (s.n + kRows - 1) / kRows,
                (s.m + kDigitTokens - 1) / kDigitTokens, (s.col_tiles + 1) / 2,
-               kRows * (int)(s.m < kDigitTokens ? s.m : kDigitTokens), 1, DigitCfg<MATS, GROUPS>::SMEM, st, y, x, w[0],
-               w[MATS - 1], s, activation, gm, dm);
+               kRows * (int)(s.m < kDigitTokens ? s.m : kDigitTokens), 1, DigitCfg<MATS, GROUPS>::SMEM, st, y, x, w,
+               MATS, s, activation, gm, dm);
 }
 
 template <int MATS>
@@ -909,6 +1281,15 @@ int run(void* y, const void* x, const W4* w, W4Shape s, int64_t m, int64_t x_row
     auto grouped = [&](auto groups) {
       constexpr int G = decltype(groups)::value;
       if (m <= kDigitTokens) return launch_digits<T, MATS, G>(y, x, w, s, activation, gm, dm, st);
+      // A launch of w4_mma_kernel starts and ends about 1 us slower, one of w4_kernel takes longer for each weight and token
+      // (us, w4_kernel and w4_mma_kernel: 4096 -> 4096 with 8 tokens 5.2 and 6.2, with 32 7.6 and 8.4, with 64 12.1 and 11.9;
+      // 14336 -> 4096 with 8 tokens 11.6 and 11.4, with 16 13.9 and 11.8, with 32 19.3 and 13.3): lines through these times
+      // cross at this many weights.
+      if (m > 32 || ((double)s.n * (double)s.k * MATS - 0x1p24) * (double)m >= 0x1p28) {
+        if (m <= 16) return launch_mma<T, MATS, 16, G>(y, x, w, s, activation, gm, dm, st);
+        if (m <= 32) return launch_mma<T, MATS, 32, G>(y, x, w, s, activation, gm, dm, st);
+        return launch_mma<T, MATS, 64, G>(y, x, w, s, activation, gm, dm, st);
+      }
       if (m <= 8) return launch<T, MATS, 1, G>(y, x, w, s, activation, gm, dm, st);
       if (m <= 16) return launch<T, MATS, 2, G>(y, x, w, s, activation, gm, dm, st);
       if (m <= 24) return launch<T, MATS, 3, G>(y, x, w, s, activation, gm, dm, st);

@@ -13,8 +13,8 @@ numbers inside the kernel that multiplies them:
 W[n, k] is ``(code - zero) * scale``; products with x are summed in fp32 and scaled in fp32, and the result is rounded
 once to the dtype of x.  Up to ``LINEAR_ROWS`` / ``GATE_UP_ROWS`` tokens take these kernels; more (a prompt) take the
 weights written out in 16 bits by ``W4Weight.dequantize`` and a library product, or the tensor-core projections of
-``fused_mlp`` / ``geglu``, whose operands then carry one more rounding (half a unit of the 16-bit type per weight).  Forward only: weights are frozen and
-an input that wants a gradient is refused.  The reference has no counterpart (its inference path is bf16,
+``fused_mlp`` / ``geglu``, whose operands then carry one more rounding (half a unit of the 16-bit type per weight).
+Forward only: weights are frozen and an input that wants a gradient is refused.  The reference has no counterpart (its inference path is bf16,
 kernels/lora_mlp/experiments/v5/lora_mlp_kernel_v5.py:451-454).  There is no path for tensors that are not on a CUDA
 device.
 """
@@ -31,10 +31,10 @@ from .swiglu import _DTYPE_CODE, _stream
 DTYPES = (torch.bfloat16, torch.float16)
 GROUP_SIZES = (32, 64, 128)
 TILE_ROWS, TILE_COLS, CODE_BYTES = 16, 128, 1024
-# Tokens up to which the 4-bit kernels are the faster side, bf16 on B200 (4-bit / 16-bit, us; the 4-bit side reads the
-# weights again for every 32 tokens).  Linear 14336 -> 4096: 36.0 / 54.8 with 64 tokens, 67.7 / 55.3 with 96; 4096 ->
-# 14336: 39.9 / 49.6 and 58.7 / 50.4.  Gate and up 4096 -> 14336: 102.4 / 116.4 with 96, 131.0 / 115.9 with 128.
-LINEAR_ROWS, GATE_UP_ROWS = 64, 96
+# Tokens up to which the 4-bit kernels are the faster side, bf16 on B200 (4-bit / 16-bit, us; the 4-bit side goes through
+# the weights again for every 64 tokens).  Linear 14336 -> 4096: 39.6 / 56.0 with 256 tokens, 70.5 / 65.9 with 384; 4096
+# -> 4096: 16.3 / 17.9 and 25.9 / 20.0.  Gate and up 4096 -> 14336: 149.3 / 154.5 with 448, 171.0 / 155.0 with 512.
+LINEAR_ROWS, GATE_UP_ROWS = 256, 448
 
 
 def _ceil(a: int, b: int) -> int:

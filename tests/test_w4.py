@@ -243,6 +243,52 @@ def test_linear(dtype, group, zeros, m, n, k):
     assert torch.equal(y, w4_linear(x, w))                # the order of every sum is fixed
 
 
+def big(n, k, group, zeros, dtype, seed=0):
+    """A weight made on the device and, of its rows, some with their float64 values: the first and last ones and a few
+    from each part."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    packed = torch.randint(0, 256, (n, 16 * ((k + 31) // 32)), generator=g, dtype=torch.uint8, device="cuda")
+    scales = ((0.5 + torch.rand(n, (k + group - 1) // group, generator=g, device="cuda")) / (4.6 * math.sqrt(k))).to(dtype)
+    z = torch.randint(0, 16, scales.shape, generator=g, dtype=torch.uint8, device="cuda") if zeros else None
+    rows = sorted({r for r in (*range(0, n, max(1, n // 90)), *range(min(n, 20)), *range(max(0, n - 150), n))})
+    part = weight64(packed[rows], scales[rows], None if z is None else z[rows], k, group)
+    return W4Weight(packed, scales, z, in_features=k, group_size=group), rows, part
+
+
+# Sizes at which the weights are many enough for the tensor-core kernel with 16, 32 and 64 tokens to a launch: few tokens,
+# full and ragged tiles of tokens, one and several of them, odd rows and columns, clusters of all kinds.
+MANY = [(3, 7001, 16000), (8, 4096, 14336), (16, 11009, 5500), (17, 9000, 4104), (32, 5503, 6000), (31, 300, 100000),
+        (33, 16, 128), (40, 1, 8), (48, 2731, 1000), (64, 129, 2048), (64, 11009, 5504), (65, 4096, 4096), (96, 5000, 136),
+        (130, 333, 264), (200, 14336, 1024), (256, 600, 96)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("group,zeros", [(128, False), (64, True), (32, False), (128, True)])
+@pytest.mark.parametrize("m,n,k", MANY)
+def test_linear_with_many_weights(dtype, group, zeros, m, n, k):
+    w, rows, w64 = big(n, k, group, zeros, dtype, seed=m)
+    x = tokens(m, k, dtype)
+    y = w4_linear(x, w)
+    assert y.shape == (m, n)
+    assert_linear(y[:, rows], x, w64, k, group)
+
+
+@gpu
+@pytest.mark.parametrize("act,gm,dm", [("silu", 0.7, 1.3), ("gelu_tanh", 1.0, 1.0), ("gelu_exact", 1.0, 1.0)])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k,group,zeros", [(5, 5120, 7000, 64, True), (8, 4096, 11008, 128, False),
+                                               (16, 11008, 2048, 32, True), (30, 4001, 4096, 128, True),
+                                               (33, 40, 264, 64, False), (64, 11008, 1024, 128, False),
+                                               (90, 2731, 1000, 32, True), (200, 500, 640, 64, True)])
+def test_gate_up_with_many_weights(act, gm, dm, dtype, m, n, k, group, zeros):
+    wg, rows, g64 = big(n, k, group, zeros, dtype, seed=m)
+    wu, _, u64 = big(n, k, group, not zeros, dtype, seed=m + 1)
+    x = tokens(m, k, dtype)
+    h = w4_gate_up(x, wg, wu, act, gm, dm)
+    assert_gate_up(h[:, rows], x, g64, u64, k, group, act, gm, dm)
+
+
 @gpu
 @pytest.mark.parametrize("act,gm,dm", [("silu", 1.0, 1.0), ("silu", 0.7, 1.3), ("gelu_tanh", 1.0, 1.0),
                                        ("gelu_exact", 1.0, 1.0)])
@@ -338,7 +384,59 @@ def test_infinities_and_nan_stay_in_their_token(dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("m,n,k", [(97, 64, 256), (150, 48, 1000), (120, 37, 129)])
+@pytest.mark.parametrize("m,n,k,offset,extra", [(40, 60, 300, 8, 20), (70, 200, 129, 0, 7), (20, 9001, 4096, 16, 8)])
+def test_many_tokens_in_pitched_rows_keep_what_is_around_them(dtype, m, n, k, offset, extra):
+    """The tokens' and the results' neighbours: NaN beside the tokens is not read, memory beside the results not written;
+    Inf and NaN stay in their tokens."""
+    w, rows, w64 = big(n, k, 64, True, dtype)
+    wide = torch.full((m + 1, offset + k + extra), float("nan"), dtype=dtype, device="cuda")
+    x = wide[:m, offset:offset + k]
+    x.copy_(tokens(m, k, dtype))
+    assert_linear(w4_linear(x, w)[:, rows], x, w64, k, 64)
+    # the C entry writes rows of any pitch
+    aligned, pitch = w4._aligned_rows(x)
+    y = torch.full((m + 2, n + 5), 7.0, dtype=dtype, device="cuda")
+    assert _lib.lib.swiglu_b200_w4_linear(y[1].data_ptr(), aligned.data_ptr(), *w._operand(), m, n, k, pitch, n + 5, 64,
+                                          CODES[dtype], 0, torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(y[1:m + 1, :n], w4_linear(x, w))
+    assert bool((y[0] == 7).all()) and bool((y[m + 1] == 7).all()) and bool((y[1:m + 1, n:] == 7).all())
+    want = w4_linear(x, w)
+    x[1, 7], x[m - 1, k - 1] = float("nan"), float("inf")
+    got = w4_linear(x, w)
+    assert bool(torch.isnan(got[1]).all()) and not bool(torch.isfinite(got[m - 1]).any())
+    keep = [i for i in range(m) if i not in (1, m - 1)]
+    assert torch.equal(got[keep], want[keep])
+
+
+@gpu
+def test_tensor_core_kernels_share_the_device():
+    """Launches of several kernels that keep their sums in tensor memory, on two streams at once: each gets its own."""
+    from kernel_pocs_b200.fused_mlp import gate_up_swiglu_forward
+
+    dtype, k = torch.bfloat16, 1024
+    w, _, _ = big(5000, k, 128, False, dtype)
+    x = tokens(64, k, dtype)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    wg, wu = (torch.randn(2048, k, generator=g, device="cuda").mul_(0.03).to(dtype) for _ in range(2))
+    with torch.no_grad():
+        want_y, want_h = w4_linear(x, w), gate_up_swiglu_forward(x, wg, wu)
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        got = [[], []]
+        for _ in range(20):
+            with torch.cuda.stream(streams[0]):
+                got[0].append(w4_linear(x, w))
+            with torch.cuda.stream(streams[1]):
+                got[1].append(gate_up_swiglu_forward(x, wg, wu))
+                got[0].append(w4_linear(x, w))
+        torch.cuda.synchronize()
+    check_status()
+    assert all(torch.equal(y, want_y) for y in got[0]) and all(torch.equal(h, want_h) for h in got[1])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(449, 64, 256), (600, 48, 1000), (512, 37, 129)])
 def test_many_tokens_take_the_16_bit_weights(dtype, m, n, k):
     """Above the limits every weight is rounded to 16 bits once more: half a unit of each product's magnitude."""
     assert m > max(w4.LINEAR_ROWS, w4.GATE_UP_ROWS)
@@ -418,7 +516,7 @@ def test_captured_token_replays_on_new_inputs_and_streams():
 
 
 @gpu
-@pytest.mark.parametrize("m", [1, 2, 8, 24])
+@pytest.mark.parametrize("m", [1, 2, 8, 24, 48, 100])
 def test_launches_in_a_row_see_what_came_before_them(m):
     """Launches may start before the one in front of them has ended: tokens, weights and outputs that change from one
     call to the next, with nothing waited for in between, against the same calls one at a time."""
