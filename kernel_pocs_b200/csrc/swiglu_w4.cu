@@ -160,17 +160,40 @@ __device__ __forceinline__ uint32_t cluster_index() {
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
-// Stores v at `addr` of the shared memory of CTA `rank` of the cluster.
-__device__ __forceinline__ void cluster_store(uint32_t addr, uint32_t rank, float v) {
+// The address of `addr` in the shared memory of CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t cluster_address(uint32_t addr, uint32_t rank) {
   uint32_t remote;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
+  return remote;
+}
+// Stores v there and counts its bytes at the barrier at `bar` there.  Waiting for that barrier ends as the last store arrives;
+// a cluster barrier that releases the stores takes 0.6 us longer, but many stores go faster uncounted (16-bit products: 128
+// rows of 3 tokens gain as much, of 12 tokens they lose it).
+__device__ __forceinline__ void cluster_send4(uint32_t addr, uint32_t bar, uint32_t rank, const float4& v) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(
+                   cluster_address(addr, rank)),
+               "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(cluster_address(bar, rank))
+               : "memory");
 }
 __device__ __forceinline__ void cluster_store4(uint32_t addr, uint32_t rank, const float4& v) {
-  uint32_t remote;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_address(addr, rank)), "f"(v.x), "f"(v.y),
+               "f"(v.z), "f"(v.w)
                : "memory");
+}
+
+// Waits for a barrier in the CTA's shared memory; false after half a second.
+__device__ __forceinline__ bool own_wait(uint64_t* bar, uint32_t parity) {
+  if (tc::mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!tc::mbar_try_wait(bar, parity))
+    if (clock64() - t0 > tc::WAIT_CYCLES) return false;
+  return true;
+}
+// A barrier for `bytes` that the cluster sends, made by one thread before the cluster's first barrier.
+__device__ __forceinline__ void expect_sums(uint64_t* bar, int bytes) {
+  tc::mbar_init(bar, 1);
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  if (bytes > 0) tc::mbar_expect_tx(bar, bytes);
 }
 
 // What a pair of projections (or one alone) comes to.
@@ -219,8 +242,8 @@ template <int MATS, int NT, int GROUPS> struct Cfg {
 
 // A CTA owns 8 row tiles (one to a warp; two would read the tokens' fragments once for both, but 128 rows to a CTA
 // balance better: fp16 32 x 5504 -> 11009 21.6 us against 23.5) of MATS matrices, 8 * NT tokens and, as rank r of a
-// cluster of `split` CTAs, the r-th part of the column tiles.  Each rank finishes a slice of the outputs: the others store their sums for
-// it into its shared memory, where they are added in a fixed order.
+// cluster of `split` CTAs, the r-th part of the column tiles.  Each rank finishes a slice of the outputs: the others store
+// their sums for it into its shared memory, where they are added in a fixed order.
 template <class T, int MATS, int NT, int GROUPS>
 __global__ void __launch_bounds__(32 * kWarps, Cfg<MATS, NT, GROUPS>::CTAS)
 w4_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, int activation, float gm, float dm) {
@@ -474,14 +497,6 @@ __device__ __forceinline__ void tile_load(uint32_t dst, const CUtensorMap& map, 
       "l"(&map), "r"(col), "r"(row), "r"(tc::smem_u32(bar))
       : "memory");
 }
-// Waits for a barrier that only this CTA's own copies or products arrive at; false after half a second.
-__device__ __forceinline__ bool own_wait(uint64_t* bar, uint32_t parity) {
-  if (tc::mbar_try_wait(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (!tc::mbar_try_wait(bar, parity))
-    if (clock64() - t0 > tc::WAIT_CYCLES) return false;
-  return true;
-}
 // True for one lane of a warp whose lanes all take part.
 __device__ __forceinline__ bool elect() {
   uint32_t one;
@@ -722,7 +737,9 @@ constexpr int kRowWarps = 4, kColWarps = kWarps / kRowWarps;  // a CTA: four row
 constexpr int kDigitOutputs = kRowWarps * kTileRows * kDigitTokens;
 
 template <int MATS, int GROUPS> struct DigitCfg {
-  static constexpr int SLOT = 2 * block_bytes(GROUPS, true);      // a pair of blocks
+  // A pair of blocks, as far from a 128-byte boundary as it is in the weights: copies between unlike places cost more (half
+  // a sector apart 1 x 4096 -> 14336 takes 16.9 us, whole sectors 13.9, this 13.5).
+  static constexpr int SLOT = (2 * block_bytes(GROUPS, true) + 127) / 128 * 128 + 128;
   static constexpr int PAIR = MATS * SLOT;
   static constexpr int DEPTH = MATS == 1 ? 4 : 2;                 // pairs of a warp in flight
   static constexpr int RING = kWarps * DEPTH * PAIR;
@@ -730,7 +747,7 @@ template <int MATS, int GROUPS> struct DigitCfg {
   static constexpr int SUMS = kSlab * GROUPS * 8 * 4;             // [tile][group][8]
   static constexpr int UNITS = kSlab / 2 * 8 * 4;                 // [pair][8]
   static constexpr int ARRIVALS = MATS * kColWarps * (kDigitOutputs + 64) * 4;  // [matrix][column warp][rank][slice]
-  static constexpr int SMEM = RING + DIGITS + SUMS + UNITS + ARRIVALS;
+  static constexpr int SMEM = RING + DIGITS + SUMS + UNITS + ARRIVALS + 16;  // the last bytes are a barrier
 };
 
 __device__ __forceinline__ void imma(uint32_t (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -768,8 +785,9 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
   using C = DigitCfg<MATS, GROUPS>;
   constexpr int DEPTH = C::DEPTH;
   extern __shared__ __align__(16) unsigned char smem[];
-  cluster_arrive();  // all CTAs of the cluster have started once this is waited for
   let_next_start();
+  // not a variable of its own, which would move all else off its 128-byte boundaries
+  uint64_t* const sums = reinterpret_cast<uint64_t*>(smem + C::SMEM - 8);
   const uint32_t smem_addr = (uint32_t)__cvta_generic_to_shared(smem);
   unsigned char* digits = smem + C::RING;
   float* digit_sums = reinterpret_cast<float*>(digits + C::DIGITS);
@@ -784,6 +802,12 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
   const long long token0 = (long long)blockIdx.y * kDigitTokens;
   const int tokens = s.m - token0 < kDigitTokens ? (int)(s.m - token0) : kDigitTokens;
   const W4 w[2] = {w0, w1};
+  constexpr int kRows = kRowWarps * kTileRows;
+  // Each rank finishes `slice` (a multiple of 4) of the outputs [token][row].
+  const int outputs = tokens * kRows, slice = s.slice;
+  const int mine = min(slice, outputs - rank * slice);
+  if (threadIdx.x == 0) expect_sums(sums, MATS * kColWarps * split * mine * 4);
+  cluster_arrive_relaxed();  // all CTAs of the cluster are ready for sums once this is waited for
 
   // This thread's eight columns of a token, of the slab that starts at pair p.
   auto read_token = [&](int p, int tok) {
@@ -845,18 +869,22 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
   const unsigned char* ring = smem + warp * (DEPTH * C::PAIR);
   const uint32_t ring_addr = smem_addr + warp * (DEPTH * C::PAIR);
   const char* src[MATS];  // the warp's next pair
+  uint32_t place[MATS];   // where the pair to read next was, modulo 2^32
 #pragma unroll
-  for (int a = 0; a < MATS; ++a)
+  for (int a = 0; a < MATS; ++a) {
     src[a] = cbyte(w[a].blocks) +
              ((long long)row_tile * s.col_tiles + 2 * (first + col_warp)) * block_bytes(GROUPS, w[a].zeros);
+    place[a] = (uint32_t)(uintptr_t)src[a];
+  }
   int fill = 0;  // offset of the slot to fill next
   auto fetch = [&](int p) {  // always one group of copies, empty past the last pair
     if (p < last && there) {
 #pragma unroll
       for (int a = 0; a < MATS; ++a) {
         const int bytes = block_bytes(GROUPS, w[a].zeros);
-        warp_copy<(C::SLOT + 511) / 512>(ring_addr + fill + a * C::SLOT, src[a], 2 * p + 1 == s.col_tiles ? bytes : 2 * bytes,
-                                         lane);
+        warp_copy<(2 * block_bytes(GROUPS, true) + 511) / 512>(
+            ring_addr + fill + a * C::SLOT + ((uint32_t)(uintptr_t)src[a] & 127u), src[a],
+            2 * p + 1 == s.col_tiles ? bytes : 2 * bytes, lane);
         src[a] += 2 * kColWarps * bytes;
       }
     }
@@ -910,7 +938,7 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
         const uint32_t b[4][2] = {{b0.x, b0.y}, {b0.z, b0.w}, {b1.x, b1.y}, {b1.z, b1.w}};
 #pragma unroll
         for (int a = 0; a < MATS; ++a) {
-          const unsigned char* slot = ring + take + a * C::SLOT + h * block_bytes(GROUPS, w[a].zeros);
+          const unsigned char* slot = ring + take + a * C::SLOT + (place[a] & 127u) + h * block_bytes(GROUPS, w[a].zeros);
           const uint4 lo4 = *reinterpret_cast<const uint4*>(slot + lane * 16);
           const uint4 hi4 = *reinterpret_cast<const uint4*>(slot + 512 + lane * 16);
           const uint32_t lo[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, hi[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
@@ -942,35 +970,38 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
         }
       }
       take = take == (DEPTH - 1) * C::PAIR ? 0 : take + C::PAIR;
+#pragma unroll
+      for (int a = 0; a < MATS; ++a) place[a] += 2 * kColWarps * block_bytes(GROUPS, w[a].zeros);
     }
   }
 
   copies_wait<0>();
   // A token's three columns, added up: token 0 is columns 0, 1, 2 and ends up in lanes t = 0, token 1 in lanes t = 1.
-  // Each rank finishes `slice` of the outputs [token][row]; what the warps have of it is stored there.
-  constexpr int kRows = kRowWarps * kTileRows;
-  const int outputs = tokens * kRows, slice = s.slice;
   const uint32_t arrivals = smem_addr + C::RING + C::DIGITS + C::SUMS + C::UNITS;
-  cluster_wait();
+  float* leaving = reinterpret_cast<float*>(smem + warp * (DEPTH * C::PAIR));  // [matrix][token][row] of this warp
 #pragma unroll
   for (int a = 0; a < MATS; ++a)
 #pragma unroll
     for (int hi = 0; hi < 2; ++hi) {
       const float c0 = acc[a][2 * hi], c1 = acc[a][2 * hi + 1];
       const float above = __shfl_down_sync(0xffffffffu, c0, 1), both = __shfl_down_sync(0xffffffffu, c0 + c1, 1);
-      const float v = t == 0 ? c0 + c1 + above : c1 + both;
-      const int o = t * kRows + row_warp * kTileRows + g + 8 * hi, owner = (int)((unsigned)o / (unsigned)slice);
-      if (t < tokens)
-        cluster_store(arrivals + ((a * kColWarps + col_warp) * (kDigitOutputs + 64) + rank * slice + o - owner * slice) * 4,
-                      owner, v);
+      if (t < tokens) leaving[(a * kDigitTokens + t) * kTileRows + g + 8 * hi] = t == 0 ? c0 + c1 + above : c1 + both;
     }
-  cluster_arrive();
+  __syncwarp();
   cluster_wait();
+  if (lane < MATS * kDigitTokens * 4) {
+    const int a = lane / (kDigitTokens * 4), tok = lane / 4 % kDigitTokens;
+    const int o = tok * kRows + row_warp * kTileRows + lane % 4 * 4, owner = (int)((unsigned)o / (unsigned)slice);
+    if (tok < tokens)
+      cluster_send4(arrivals + ((a * kColWarps + col_warp) * (kDigitOutputs + 64) + rank * slice + o - owner * slice) * 4,
+                    tc::smem_u32(sums), owner, *reinterpret_cast<const float4*>(leaving + lane * 4));
+  }
+  const bool there_in_time = mine <= 0 || own_wait(sums, 0);
   const float* parts = reinterpret_cast<const float*>(smem + C::RING + C::DIGITS + C::SUMS + C::UNITS);
-  const int begin = rank * slice, o = threadIdx.x;  // slice <= kDigitOutputs <= 32 * kWarps
+  const int begin = rank * slice, o = threadIdx.x;  // mine <= kDigitOutputs <= 32 * kWarps
   const int row = (begin + o) % kRows, tok = (begin + o) / kRows;
   const long long n = (long long)row_tile0 * kTileRows + row;
-  if (o < slice && begin + o < outputs && n < s.n) {
+  if (o < mine && n < s.n) {
     float v[MATS];
 #pragma unroll
     for (int a = 0; a < MATS; ++a) {
@@ -980,6 +1011,7 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
 #pragma unroll
         for (int q = 0; q < kColWarps; ++q) v[a] += parts[(a * kColWarps + q) * (kDigitOutputs + 64) + i * slice + o];
     }
+    if (!there_in_time) v[0] = __uint_as_float(0x7fffffffu);
     const Consts consts(gm, dm);
     static_cast<uint16_t*>(y)[(token0 + tok) * s.y_pitch + n] = H::from_float(result<MATS>(v, activation, consts));
   }
@@ -1251,7 +1283,7 @@ int launch_digits(void* y, const void* x, const W4* w, const W4Shape& s, int act
   static Launcher known;
   return start(w4_digits_kernel<T, MATS, GROUPS>, known, (s.n + kRows - 1) / kRows,
                (s.m + kDigitTokens - 1) / kDigitTokens, (s.col_tiles + 1) / 2,
-               kRows * (int)(s.m < kDigitTokens ? s.m : kDigitTokens), 1, DigitCfg<MATS, GROUPS>::SMEM, st, y, x, w,
+               kRows * (int)(s.m < kDigitTokens ? s.m : kDigitTokens), 4, DigitCfg<MATS, GROUPS>::SMEM, st, y, x, w,
                MATS, s, activation, gm, dm);
 }
 
