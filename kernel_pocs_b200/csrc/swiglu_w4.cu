@@ -732,11 +732,10 @@ w4_mma_kernel(void* y, const __grid_constant__ Maps maps, W4 w0, W4 w1, W4Shape 
 
 constexpr int kDigitTokens = 2, kDigitCols = 3 * kDigitTokens;
 constexpr int kSlab = 16;                              // column tiles whose digits are kept at a time, in pairs
-constexpr int kRowWarps = 4, kColWarps = kWarps / kRowWarps;  // a CTA: four row tiles, the tile pairs dealt to two warps
 
-constexpr int kDigitOutputs = kRowWarps * kTileRows * kDigitTokens;
-
-template <int MATS, int GROUPS> struct DigitCfg {
+// A CTA: ROW_WARPS row tiles, whose pairs of column tiles are dealt to the warps that are left over.
+template <int MATS, int GROUPS, int ROW_WARPS> struct DigitCfg {
+  static constexpr int COL_WARPS = kWarps / ROW_WARPS, OUTPUTS = ROW_WARPS * kTileRows * kDigitTokens;
   // A pair of blocks, as far from a 128-byte boundary as it is in the weights: copies between unlike places cost more (half
   // a sector apart 1 x 4096 -> 14336 takes 16.9 us, whole sectors 13.9, this 13.5).
   static constexpr int SLOT = (2 * block_bytes(GROUPS, true) + 127) / 128 * 128 + 128;
@@ -746,7 +745,7 @@ template <int MATS, int GROUPS> struct DigitCfg {
   static constexpr int DIGITS = kSlab * 2 * kDigitCols * 4 * 16;  // [tile][2][column][t] 16 bytes
   static constexpr int SUMS = kSlab * GROUPS * 8 * 4;             // [tile][group][8]
   static constexpr int UNITS = kSlab / 2 * 8 * 4;                 // [pair][8]
-  static constexpr int ARRIVALS = MATS * kColWarps * (kDigitOutputs + 64) * 4;  // [matrix][column warp][rank][slice]
+  static constexpr int ARRIVALS = MATS * COL_WARPS * (OUTPUTS + 64) * 4;  // [matrix][column warp][rank][slice]
   static constexpr int SMEM = RING + DIGITS + SUMS + UNITS + ARRIVALS + 16;  // the last bytes are a barrier
 };
 
@@ -775,15 +774,15 @@ template <> __device__ __forceinline__ uint32_t top_of<__half>(const Vec<16>& v)
 constexpr float kIntMagic = 12582912.0f;  // 1.5 * 2^23: added to an integer below 2^22, its bits are 0x4b400000 + it
 constexpr uint32_t kIntMagicBits = 0x4b400000u;
 
-// A CTA owns kRowWarps row tiles of MATS matrices, up to two tokens and, as rank r of a cluster of `split` CTAs, the
+// A CTA owns ROW_WARPS row tiles of MATS matrices, up to two tokens and, as rank r of a cluster of `split` CTAs, the
 // r-th part of the pairs of column tiles.  The code is kept short (loops that are not unrolled): a launch lasts a few
 // microseconds, most of its instructions run once, and a start waits for them to be fetched.
-template <class T, int MATS, int GROUPS>
+template <class T, int MATS, int GROUPS, int ROW_WARPS>
 __global__ void __launch_bounds__(32 * kWarps, 2)
 w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, int activation, float gm, float dm) {
   using H = Half2<T>;
-  using C = DigitCfg<MATS, GROUPS>;
-  constexpr int DEPTH = C::DEPTH;
+  using C = DigitCfg<MATS, GROUPS, ROW_WARPS>;
+  constexpr int DEPTH = C::DEPTH, COL_WARPS = C::COL_WARPS;
   extern __shared__ __align__(16) unsigned char smem[];
   let_next_start();
   // not a variable of its own, which would move all else off its 128-byte boundaries
@@ -794,19 +793,19 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
   float* units = reinterpret_cast<float*>(digits + C::DIGITS + C::SUMS);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int row_warp = warp % kRowWarps, col_warp = warp / kRowWarps;
+  const int row_warp = warp % ROW_WARPS, col_warp = warp / ROW_WARPS;
   const int rank = (int)cluster_rank(), split = s.split;
   const int first = rank * s.share + min(rank, s.over), last = first + s.share + (rank < s.over ? 1 : 0);  // pairs
-  const int row_tile0 = (int)cluster_index() * kRowWarps, row_tile = row_tile0 + row_warp;  // of the CTA, the warp
+  const int row_tile0 = (int)cluster_index() * ROW_WARPS, row_tile = row_tile0 + row_warp;  // of the CTA, the warp
   const bool there = (long long)row_tile * kTileRows < s.n;
   const long long token0 = (long long)blockIdx.y * kDigitTokens;
   const int tokens = s.m - token0 < kDigitTokens ? (int)(s.m - token0) : kDigitTokens;
   const W4 w[2] = {w0, w1};
-  constexpr int kRows = kRowWarps * kTileRows;
+  constexpr int kRows = ROW_WARPS * kTileRows;
   // Each rank finishes `slice` (a multiple of 4) of the outputs [token][row].
   const int outputs = tokens * kRows, slice = s.slice;
   const int mine = min(slice, outputs - rank * slice);
-  if (threadIdx.x == 0) expect_sums(sums, MATS * kColWarps * split * mine * 4);
+  if (threadIdx.x == 0) expect_sums(sums, MATS * COL_WARPS * split * mine * 4);
   cluster_arrive_relaxed();  // all CTAs of the cluster are ready for sums once this is waited for
 
   // This thread's eight columns of a token, of the slab that starts at pair p.
@@ -885,7 +884,7 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
         warp_copy<(2 * block_bytes(GROUPS, true) + 511) / 512>(
             ring_addr + fill + a * C::SLOT + ((uint32_t)(uintptr_t)src[a] & 127u), src[a],
             2 * p + 1 == s.col_tiles ? bytes : 2 * bytes, lane);
-        src[a] += 2 * kColWarps * bytes;
+        src[a] += 2 * COL_WARPS * bytes;
       }
     }
     copies_commit();
@@ -895,14 +894,14 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
   if (lane < MATS && there && first < last) {
     const W4& mine = lane == 0 ? w0 : w1;
     const int bytes = block_bytes(GROUPS, mine.zeros);
-    // both column warps of a row ask for the same few pairs
+    // the column warps of a row ask for the same few pairs
     prefetch_l2(cbyte(mine.blocks) + ((long long)row_tile * s.col_tiles + 2 * first) * bytes,
-                min((DEPTH - 1) * kColWarps * 2, min(2 * last, s.col_tiles) - 2 * first) * bytes);
+                min((DEPTH - 1) * COL_WARPS * 2, min(2 * last, s.col_tiles) - 2 * first) * bytes);
   }
   wait_for_previous();
   Vec<16> token = read_token(first, 0);
 #pragma unroll 1
-  for (int i = 0; i < DEPTH - 1; ++i) fetch(first + col_warp + i * kColWarps);
+  for (int i = 0; i < DEPTH - 1; ++i) fetch(first + col_warp + i * COL_WARPS);
 
   float acc[MATS][4] = {};
   int take = 0;  // offset of the slot to read next
@@ -921,10 +920,10 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
     __syncthreads();
     const int end = last < slab + kSlab / 2 ? last : slab + kSlab / 2;
 #pragma unroll 1
-    for (int p = slab + col_warp; p < end; p += kColWarps) {
+    for (int p = slab + col_warp; p < end; p += COL_WARPS) {
       copies_wait<DEPTH - 2>();
       __syncwarp();  // this pair is there for all lanes, and the one before has been read by all
-      fetch(p + (DEPTH - 1) * kColWarps);
+      fetch(p + (DEPTH - 1) * COL_WARPS);
       if (!there) continue;
       const float2 unit = *reinterpret_cast<const float2*>(units + (p - slab) * 8 + 2 * t);
 #pragma unroll
@@ -971,7 +970,7 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
       }
       take = take == (DEPTH - 1) * C::PAIR ? 0 : take + C::PAIR;
 #pragma unroll
-      for (int a = 0; a < MATS; ++a) place[a] += 2 * kColWarps * block_bytes(GROUPS, w[a].zeros);
+      for (int a = 0; a < MATS; ++a) place[a] += 2 * COL_WARPS * block_bytes(GROUPS, w[a].zeros);
     }
   }
 
@@ -993,12 +992,12 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
     const int a = lane / (kDigitTokens * 4), tok = lane / 4 % kDigitTokens;
     const int o = tok * kRows + row_warp * kTileRows + lane % 4 * 4, owner = (int)((unsigned)o / (unsigned)slice);
     if (tok < tokens)
-      cluster_send4(arrivals + ((a * kColWarps + col_warp) * (kDigitOutputs + 64) + rank * slice + o - owner * slice) * 4,
+      cluster_send4(arrivals + ((a * COL_WARPS + col_warp) * (C::OUTPUTS + 64) + rank * slice + o - owner * slice) * 4,
                     tc::smem_u32(sums), owner, *reinterpret_cast<const float4*>(leaving + lane * 4));
   }
   const bool there_in_time = mine <= 0 || own_wait(sums, 0);
   const float* parts = reinterpret_cast<const float*>(smem + C::RING + C::DIGITS + C::SUMS + C::UNITS);
-  const int begin = rank * slice, o = threadIdx.x;  // mine <= kDigitOutputs <= 32 * kWarps
+  const int begin = rank * slice, o = threadIdx.x;  // mine <= OUTPUTS <= 32 * kWarps
   const int row = (begin + o) % kRows, tok = (begin + o) / kRows;
   const long long n = (long long)row_tile0 * kTileRows + row;
   if (o < mine && n < s.n) {
@@ -1009,7 +1008,7 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
 #pragma unroll 1
       for (int i = 0; i < split; ++i)
 #pragma unroll
-        for (int q = 0; q < kColWarps; ++q) v[a] += parts[(a * kColWarps + q) * (kDigitOutputs + 64) + i * slice + o];
+        for (int q = 0; q < COL_WARPS; ++q) v[a] += parts[(a * COL_WARPS + q) * (C::OUTPUTS + 64) + i * slice + o];
     }
     if (!there_in_time) v[0] = __uint_as_float(0x7fffffffu);
     const Consts consts(gm, dm);
@@ -1170,7 +1169,8 @@ template <class X> struct Start {
     cfg.attrs = attrs;
     return SWIGLU_B200_OK;
   }
-  // How many clusters of `split` CTAs run at once; negative: an error code.
+  // How many clusters of `split` CTAs run at once, with a few places left free (with every one taken 1 x 8192 -> 3584 took
+  // 7.3 us, not 5.4); negative: an error code.
   int at_once(int split) {
     int n = device < 64 ? known.clusters[device][split].load(std::memory_order_relaxed) : 0;
     if (n == 0) {
@@ -1181,7 +1181,7 @@ template <class X> struct Start {
       if (e != cudaSuccess) return -note_cuda_error(SWIGLU_B200_ERR_DEVICE, e);
       if (device < 64) known.clusters[device][split].store(n, std::memory_order_relaxed);
     }
-    return n;
+    return n - n / 32;
   }
   int launch(long long clusters, long long gy, void* y, const X& x, const W4* w, int mats, const W4Shape& s, int activation,
              float gm, float dm) {
@@ -1276,16 +1276,18 @@ int launch_mma(void* y, const void* x, const W4* w, const W4Shape& s, int activa
   return k.launch((row_groups + groups - 1) / groups, gy, y, maps, w, MATS, shape, activation, gm, dm);
 }
 
-template <class T, int MATS, int GROUPS>
+template <class T, int MATS, int GROUPS, int ROW_WARPS>
 int launch_digits(void* y, const void* x, const W4* w, const W4Shape& s, int activation, float gm, float dm,
                   cudaStream_t st) {
-  constexpr int kRows = kRowWarps * kTileRows;
+  constexpr int kRows = ROW_WARPS * kTileRows;
   static Launcher known;
-  return start(w4_digits_kernel<T, MATS, GROUPS>, known, (s.n + kRows - 1) / kRows,
+  return start(w4_digits_kernel<T, MATS, GROUPS, ROW_WARPS>, known, (s.n + kRows - 1) / kRows,
                (s.m + kDigitTokens - 1) / kDigitTokens, (s.col_tiles + 1) / 2,
-               kRows * (int)(s.m < kDigitTokens ? s.m : kDigitTokens), 4, DigitCfg<MATS, GROUPS>::SMEM, st, y, x, w,
+               kRows * (int)(s.m < kDigitTokens ? s.m : kDigitTokens), 4, DigitCfg<MATS, GROUPS, ROW_WARPS>::SMEM, st, y, x, w,
                MATS, s, activation, gm, dm);
 }
+
+constexpr int kEnoughCtas = 192;  // one to a SM and some more
 
 template <int MATS>
 int run(void* y, const void* x, const W4* w, W4Shape s, int64_t m, int64_t x_row_stride, int64_t y_row_stride,
@@ -1312,7 +1314,15 @@ int run(void* y, const void* x, const W4* w, W4Shape s, int64_t m, int64_t x_row
     using T = decltype(t);
     auto grouped = [&](auto groups) {
       constexpr int G = decltype(groups)::value;
-      if (m <= kDigitTokens) return launch_digits<T, MATS, G>(y, x, w, s, activation, gm, dm, st);
+      if (m <= kDigitTokens) {
+        // 128 rows to a CTA leave it a shorter part of the tokens to make digits of, and can be split more evenly; 64 rows
+        // make more CTAs where there are few rows, and smaller clusters (us, 64 and 128: 1 x 5504 -> 11009 11.6 and 8.2, 14336 ->
+        // 4096 8.7 and 7.6, 4096 -> 4096 3.9 and 3.9, gate and up 2048 -> 4096 3.9 and 4.4, 8192 -> 2048 4.0 and 5.1).
+        const long long pairs = (s.col_tiles + 1) / 2;
+        if (pairs >= 16 && (s.n + 127) / 128 * 8 >= kEnoughCtas)
+          return launch_digits<T, MATS, G, 8>(y, x, w, s, activation, gm, dm, st);
+        return launch_digits<T, MATS, G, 4>(y, x, w, s, activation, gm, dm, st);
+      }
       // A launch of w4_mma_kernel starts and ends about 1 us slower, one of w4_kernel takes longer for each weight and token
       // (us, w4_kernel and w4_mma_kernel: 4096 -> 4096 with 8 tokens 5.2 and 6.2, with 32 7.6 and 8.4, with 64 12.1 and 11.9;
       // 14336 -> 4096 with 8 tokens 11.6 and 11.4, with 16 13.9 and 11.8, with 32 19.3 and 13.3): lines through these times
