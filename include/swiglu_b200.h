@@ -335,7 +335,7 @@ SWIGLU_B200_API int swiglu_b200_ckpt8_bwd(void* h, void* dgate, void* dup, const
                           int64_t cols, int64_t grad_row_stride, int64_t dout_row_stride, int64_t h_row_stride,
                           int dtype, int activation, float gm, float dm, int device, void* stream);
 
-/* Projections with 4-bit weights for a few tokens, forward only; fp16 or bf16 tokens, results and scales.  No
+/* Projections with 4-bit weights, forward only; fp16 or bf16 tokens, results and scales.  No
  * counterpart in the reference, whose inference path keeps 16-bit weights.
  *
  *   linear    y[m][n] = sum_k x[m][k] * (q[n][k] - z[n][k/group]) * s[n][k/group]
@@ -354,9 +354,10 @@ SWIGLU_B200_API int swiglu_b200_ckpt8_bwd(void* h, void* dgate, void* dup, const
  *   x        m x k, row stride x_row_stride; 16-byte aligned rows (a stride that is a multiple of 8 when m > 1)
  *   y, h     m x n, row stride given; may not overlap x or the weights
  *   group    32, 64 or 128 columns share a scale
- * Meant for m up to a few tens: every 32 tokens read the weights again.  One or two tokens are multiplied as 23-bit
- * integers relative to the largest magnitude of their 256 columns (a token with an Inf or a NaN gives NaN); more go
- * through 16-bit products.  The order of every sum is fixed.
+ * Meant for m up to a few hundred: every 64 tokens go through the weights again.  n and k are at most 2^30.  One or two
+ * tokens are multiplied as 23-bit integers relative to the largest magnitude of their 256 columns (a token with an Inf or
+ * a NaN gives NaN); more go through 16-bit products.  The order of every sum is fixed.  A wait inside a kernel that gives
+ * up, after half a second, turns the results of its CTA to NaN.
  * A call's kernel may start while the kernel of the linear / gate_up call before it on the stream is finishing; it reads
  * and writes nothing of the caller's until everything enqueued earlier is complete. */
 SWIGLU_B200_API int swiglu_b200_w4_linear(void* y, const void* x, const void* blocks, int zeros, int64_t m, int64_t n,

@@ -241,7 +241,7 @@ template <int MATS, int NT, int GROUPS> struct Cfg {
 };
 
 // A CTA owns 8 row tiles (one to a warp; two would read the tokens' fragments once for both, but 128 rows to a CTA
-// balance better: fp16 32 x 5504 -> 11009 21.6 us against 23.5) of MATS matrices, 8 * NT tokens and, as rank r of a
+// balance better: fp16 32 x 5504 -> 11009 21.6 us against 23.5) of MATS matrices, up to 8 * NT tokens and, as rank r of a
 // cluster of `split` CTAs, the r-th part of the column tiles.  Each rank finishes a slice of the outputs: the others store
 // their sums for it into its shared memory, where they are added in a fixed order.
 template <class T, int MATS, int NT, int GROUPS>
@@ -258,7 +258,6 @@ w4_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, int acti
   const int rank = (int)cluster_rank(), split = s.split;
   const int row_tiles = (int)((s.n + kTileRows - 1) / kTileRows);
   const int row_tile0 = (int)cluster_index() * kWarps, row_tile = row_tile0 + warp;  // of the CTA, the warp
-  const long long token0 = (long long)blockIdx.y * (8 * NT);
   const int first = rank * s.share + min(rank, s.over), last = first + s.share + (rank < s.over ? 1 : 0);
   const W4 w[2] = {w0, w1};
 
@@ -272,8 +271,8 @@ w4_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, int acti
   for (int i = 0; i < ROUNDS; ++i) {
     const int o = threadIdx.x + i * 32 * kWarps, tok = o >> 4, piece = o & 15;
     const long long k = (long long)first * kTileCols + 8 * piece;
-    const bool mine = o < PIECES && token0 + tok < s.m;
-    x_src[i] = mine ? cbyte(x) + ((token0 + tok) * s.x_pitch + k) * 2 : cbyte(x);
+    const bool mine = o < PIECES && tok < s.m;
+    x_src[i] = mine ? cbyte(x) + (tok * s.x_pitch + k) * 2 : cbyte(x);
     x_left[i] = mine ? (s.k - k) * 2 : 0;
   }
   int fill = 0;  // offset of the stage to fill next
@@ -397,7 +396,7 @@ w4_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, int acti
   __syncthreads();
 
   // Of the outputs [token][row] that exist each rank finishes `slice` (a multiple of 4).
-  const int tokens = s.m - token0 < 8 * NT ? (int)(s.m - token0) : 8 * NT, outputs = tokens * kRows, slice = s.slice;
+  const int outputs = (int)s.m * kRows, slice = s.slice;
   const float* arrived = reinterpret_cast<const float*>(smem + DEPTH * C::STAGE);
   const int begin = split > 1 ? rank * slice : 0;
   if (split > 1) {
@@ -432,7 +431,7 @@ w4_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, int acti
       }
       v[0][a] = f.x, v[1][a] = f.y, v[2][a] = f.z, v[3][a] = f.w;
     }
-    store_results<T, MATS>(y, (token0 + tok) * s.y_pitch, n, s, v, activation, consts);
+    store_results<T, MATS>(y, tok * s.y_pitch, n, s, v, activation, consts);
   }
 }
 
@@ -798,8 +797,7 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
   const int first = rank * s.share + min(rank, s.over), last = first + s.share + (rank < s.over ? 1 : 0);  // pairs
   const int row_tile0 = (int)cluster_index() * ROW_WARPS, row_tile = row_tile0 + row_warp;  // of the CTA, the warp
   const bool there = (long long)row_tile * kTileRows < s.n;
-  const long long token0 = (long long)blockIdx.y * kDigitTokens;
-  const int tokens = s.m - token0 < kDigitTokens ? (int)(s.m - token0) : kDigitTokens;
+  const int tokens = (int)s.m;
   const W4 w[2] = {w0, w1};
   constexpr int kRows = ROW_WARPS * kTileRows;
   // Each rank finishes `slice` (a multiple of 4) of the outputs [token][row].
@@ -811,7 +809,7 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
   // This thread's eight columns of a token, of the slab that starts at pair p.
   auto read_token = [&](int p, int tok) {
     const long long k = (long long)p * (2 * kTileCols) + 8 * threadIdx.x;
-    const char* src = cbyte(x) + ((token0 + tok) * s.x_pitch + k) * 2;
+    const char* src = cbyte(x) + (tok * s.x_pitch + k) * 2;
     Vec<16> v{};
     if (k + 8 <= s.k) {
       v = Ld<16, LD_PLAIN>::ld(src);
@@ -1012,7 +1010,7 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
     }
     if (!there_in_time) v[0] = __uint_as_float(0x7fffffffu);
     const Consts consts(gm, dm);
-    static_cast<uint16_t*>(y)[(token0 + tok) * s.y_pitch + n] = H::from_float(result<MATS>(v, activation, consts));
+    static_cast<uint16_t*>(y)[tok * s.y_pitch + n] = H::from_float(result<MATS>(v, activation, consts));
   }
 }
 
@@ -1198,14 +1196,14 @@ template <class X> struct Start {
   }
 };
 
-// Launches `kernel` with one cluster for each of `clusters` x `gy`.  Its `parts` column tiles (or pairs) are split over
+// Launches `kernel` with `clusters` clusters.  Its `parts` column tiles (or pairs) are split over
 // the CTAs of a cluster, as many as leave every cluster running at once: all of them stream from the start and end
 // together (one cluster more than fit is another round, 430 CTAs instead of 258 took 22.8 us instead of 19.9).
 // `outputs` are a cluster's, finished in slices of a multiple of `unit`.
-int start(Kernel<const void*> kernel, Launcher& known, long long clusters, long long gy, int parts, int outputs, int unit,
-          int smem, cudaStream_t st, void* y, const void* x, const W4* w, int mats, W4Shape s, int activation, float gm,
+int start(Kernel<const void*> kernel, Launcher& known, long long clusters, int parts, int outputs, int unit, int smem,
+          cudaStream_t st, void* y, const void* x, const W4* w, int mats, W4Shape s, int activation, float gm,
           float dm) {
-  if (clusters > 0x7fffffffLL / 8 || gy > 65535) return SWIGLU_B200_ERR_SHAPE;
+  if (clusters > 0x7fffffffLL / 8) return SWIGLU_B200_ERR_SHAPE;
   Start<const void*> k(kernel, known, 32 * kWarps, smem);
   int rc = k.prepare(st);
   if (rc != SWIGLU_B200_OK) return rc;
@@ -1213,22 +1211,21 @@ int start(Kernel<const void*> kernel, Launcher& known, long long clusters, long 
   for (; split > 1; --split) {
     const int at_once = k.at_once(split);
     if (at_once < 0) return -at_once;
-    if (clusters * gy <= at_once) break;
+    if (clusters <= at_once) break;
   }
   s.split = split;
   s.share = parts / split;
   s.over = parts % split;
   s.slice = (outputs + unit * split - 1) / (unit * split) * unit;
-  return k.launch(clusters, gy, y, x, w, mats, s, activation, gm, dm);
+  return k.launch(clusters, 1, y, x, w, mats, s, activation, gm, dm);
 }
 
 template <class T, int MATS, int NT, int GROUPS>
 int launch(void* y, const void* x, const W4* w, const W4Shape& s, int activation, float gm, float dm, cudaStream_t st) {
   constexpr int kRows = kWarps * kTileRows;
   static Launcher known;
-  return start(w4_kernel<T, MATS, NT, GROUPS>, known, (s.n + kRows - 1) / kRows, (s.m + 8 * NT - 1) / (8 * NT),
-               s.col_tiles, kRows * (int)(s.m < 8 * NT ? s.m : 8 * NT), 4, Cfg<MATS, NT, GROUPS>::SMEM, st, y, x, w,
-               MATS, s, activation, gm, dm);
+  return start(w4_kernel<T, MATS, NT, GROUPS>, known, (s.n + kRows - 1) / kRows, s.col_tiles, kRows * (int)s.m, 4,
+               Cfg<MATS, NT, GROUPS>::SMEM, st, y, x, w, MATS, s, activation, gm, dm);
 }
 
 template <class T, int MATS, int N, int GROUPS>
@@ -1281,10 +1278,8 @@ int launch_digits(void* y, const void* x, const W4* w, const W4Shape& s, int act
                   cudaStream_t st) {
   constexpr int kRows = ROW_WARPS * kTileRows;
   static Launcher known;
-  return start(w4_digits_kernel<T, MATS, GROUPS, ROW_WARPS>, known, (s.n + kRows - 1) / kRows,
-               (s.m + kDigitTokens - 1) / kDigitTokens, (s.col_tiles + 1) / 2,
-               kRows * (int)(s.m < kDigitTokens ? s.m : kDigitTokens), 4, DigitCfg<MATS, GROUPS, ROW_WARPS>::SMEM, st, y, x, w,
-               MATS, s, activation, gm, dm);
+  return start(w4_digits_kernel<T, MATS, GROUPS, ROW_WARPS>, known, (s.n + kRows - 1) / kRows, (s.col_tiles + 1) / 2,
+               kRows * (int)s.m, 4, DigitCfg<MATS, GROUPS, ROW_WARPS>::SMEM, st, y, x, w, MATS, s, activation, gm, dm);
 }
 
 constexpr int kEnoughCtas = 192;  // one to a SM and some more
@@ -1316,18 +1311,18 @@ int run(void* y, const void* x, const W4* w, W4Shape s, int64_t m, int64_t x_row
       constexpr int G = decltype(groups)::value;
       if (m <= kDigitTokens) {
         // 128 rows to a CTA leave it a shorter part of the tokens to make digits of, and can be split more evenly; 64 rows
-        // make more CTAs where there are few rows, and smaller clusters (us, 64 and 128: 1 x 5504 -> 11009 11.6 and 8.2, 14336 ->
-        // 4096 8.7 and 7.6, 4096 -> 4096 3.9 and 3.9, gate and up 2048 -> 4096 3.9 and 4.4, 8192 -> 2048 4.0 and 5.1).
+        // make more CTAs where there are few rows, and smaller clusters (us, 64 and 128: 1 x 5504 -> 11009 11.6 and 8.2,
+        // 14336 -> 4096 8.7 and 7.6, 4096 -> 4096 3.9 and 3.9, gate and up 2048 -> 4096 3.9 and 4.4, 8192 -> 2048 4.0 and 5.1).
         const long long pairs = (s.col_tiles + 1) / 2;
         if (pairs >= 16 && (s.n + 127) / 128 * 8 >= kEnoughCtas)
           return launch_digits<T, MATS, G, 8>(y, x, w, s, activation, gm, dm, st);
         return launch_digits<T, MATS, G, 4>(y, x, w, s, activation, gm, dm, st);
       }
-      // A launch of w4_mma_kernel starts and ends about 1 us slower, one of w4_kernel takes longer for each weight and token
+      // A launch of w4_mma_kernel starts and ends about 1 us slower, one of w4_kernel takes longer for each weight and 8 tokens
       // (us, w4_kernel and w4_mma_kernel: 4096 -> 4096 with 8 tokens 5.2 and 6.2, with 32 7.6 and 8.4, with 64 12.1 and 11.9;
       // 14336 -> 4096 with 8 tokens 11.6 and 11.4, with 16 13.9 and 11.8, with 32 19.3 and 13.3): lines through these times
       // cross at this many weights.
-      if (m > 32 || ((double)s.n * (double)s.k * MATS - 0x1p24) * (double)m >= 0x1p28) {
+      if (m > 32 || ((double)s.n * (double)s.k * MATS - 0x1p24) * (double)((m + 7) / 8 * 8) >= 0x1p28) {
         if (m <= 16) return launch_mma<T, MATS, 16, G>(y, x, w, s, activation, gm, dm, st);
         if (m <= 32) return launch_mma<T, MATS, 32, G>(y, x, w, s, activation, gm, dm, st);
         return launch_mma<T, MATS, 64, G>(y, x, w, s, activation, gm, dm, st);

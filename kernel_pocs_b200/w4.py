@@ -1,4 +1,4 @@
-"""Gated MLP with 4-bit weights for a few tokens: the frozen projections of a block that generates.
+"""Gated MLP with 4-bit weights for one to a few hundred tokens: the frozen projections of a block that generates.
 
 With one token, or one per sequence of a small batch, an MLP costs what it takes to read its weights.  Here they are
 4-bit codes with a scale (and, optionally, a zero point) for every ``group_size`` columns, and are turned back into
@@ -268,7 +268,7 @@ def w4_linear(x: torch.Tensor, weight: W4Weight) -> torch.Tensor:
 
 
 def _gate_up_16bit(x, w_gate, w_up, activation, gm, dm):
-    """The same stage from weights written out in 16 bits, for more tokens than the 4-bit kernel is for."""
+    """The same stage from weights written out in 16 bits, for more tokens than the 4-bit kernels are for."""
     from .fused_mlp import gate_up_swiglu_forward
     from .geglu import gate_up_geglu_forward, geglu_forward
     from .swiglu import swiglu_forward
