@@ -276,7 +276,8 @@ def _gate_up_16bit(x, w_gate, w_up, activation, gm, dm):
     wg, wu = w_gate.dequantize(), w_up.dequantize()
     n, k = wg.shape
     approximate = "tanh" if activation == "gelu_tanh" else "none"
-    if x.dtype == torch.bfloat16 and k % 8 == 0 and n % 16 == 0:
+    # the fused projections report through status words that belong to launches, not to a graph's replays
+    if x.dtype == torch.bfloat16 and k % 8 == 0 and n % 16 == 0 and not torch.cuda.is_current_stream_capturing():
         if activation == "silu":
             return gate_up_swiglu_forward(x, wg, wu, gm, dm)
         return gate_up_geglu_forward(x, wg, wu, approximate)

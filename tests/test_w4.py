@@ -516,6 +516,32 @@ def test_captured_token_replays_on_new_inputs_and_streams():
 
 
 @gpu
+@pytest.mark.parametrize("m", [64, 450])
+def test_captured_gate_up_of_many_tokens(m):
+    """Also above the limit, after and between eager calls of the fused projections it takes outside a graph."""
+    dtype, n, k = torch.bfloat16, 64, 256
+    wg, _ = make(n, k, 64, True, dtype)
+    wu, _ = make(n, k, 64, False, dtype, seed=9)
+    x = tokens(m, k, dtype)
+    with torch.no_grad():
+        for _ in range(300):
+            w4_gate_up(x, wg, wu)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = [w4_gate_up(x, wg, wu) for _ in range(300)]
+        x.copy_(tokens(m, k, dtype, seed=5))
+        graph.replay()
+        eager = w4_gate_up(x, wg, wu)
+        torch.cuda.synchronize()
+    check_status()
+    assert all(torch.equal(o, outs[0]) for o in outs)
+    # projections rounded to bf16 on one side at most: two half units each, and one of the result
+    scale = float(eager.float().abs().max())
+    assert float((outs[0].float() - eager.float()).abs().max()) <= 6 * torch.finfo(dtype).eps / 2 * scale
+
+
+@gpu
 @pytest.mark.parametrize("m", [1, 2, 8, 24, 48, 100])
 def test_launches_in_a_row_see_what_came_before_them(m):
     """Launches may start before the one in front of them has ended: tokens, weights and outputs that change from one
