@@ -167,8 +167,7 @@ __device__ __forceinline__ uint32_t cluster_address(uint32_t addr, uint32_t rank
   return remote;
 }
 // Stores v there and counts its bytes at the barrier at `bar` there.  Waiting for that barrier ends as the last store arrives;
-// a cluster barrier that releases the stores takes 0.6 us longer, but many stores go faster uncounted (16-bit products: 128
-// rows of 3 tokens gain as much, of 12 tokens they lose it).
+// a cluster barrier that releases the stores takes 0.6 us longer, but many stores go faster uncounted.
 __device__ __forceinline__ void cluster_send4(uint32_t addr, uint32_t bar, uint32_t rank, const float4& v) {
   asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(
                    cluster_address(addr, rank)),
@@ -235,7 +234,7 @@ template <int MATS, int NT, int GROUPS> struct Cfg {
   static constexpr int ARRIVALS = MATS * (OUTPUTS + 64) * 4;
   static constexpr int FIT = (220 * 1024 / CTAS - ARRIVALS) / STAGE;
   static constexpr int DEPTH = FIT < 3 ? 3 : FIT > 8 ? 8 : FIT;
-  static constexpr int SMEM = DEPTH * STAGE + ARRIVALS;
+  static constexpr int SMEM = DEPTH * STAGE + ARRIVALS + 16;  // the last bytes are a barrier
   static_assert(MATS * 8 * NT * (kWarps * kTileRows + 4) * 4 <= DEPTH * STAGE,
                 "the sums on their way out reuse the stages");
 };
@@ -251,7 +250,6 @@ w4_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, int acti
   using C = Cfg<MATS, NT, GROUPS>;
   constexpr int DEPTH = C::DEPTH, PIECES = 8 * NT * 16, ROUNDS = (PIECES + 32 * kWarps - 1) / (32 * kWarps);
   extern __shared__ __align__(16) unsigned char smem[];
-  cluster_arrive();  // all CTAs of the cluster have started once this is waited for
   let_next_start();
   const uint32_t smem_addr = (uint32_t)__cvta_generic_to_shared(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -260,6 +258,16 @@ w4_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, int acti
   const int row_tile0 = (int)cluster_index() * kWarps, row_tile = row_tile0 + warp;  // of the CTA, the warp
   const int first = rank * s.share + min(rank, s.over), last = first + s.share + (rank < s.over ? 1 : 0);
   const W4 w[2] = {w0, w1};
+  // Of the outputs [token][row] that exist each rank finishes `slice` (a multiple of 4).
+  constexpr int kRows = kWarps * kTileRows, OUTPUTS = C::OUTPUTS;
+  const int outputs = (int)s.m * kRows, slice = s.slice, mine = min(slice, outputs - rank * slice);
+  // Whether sums travel as counted stores (us for 4096 -> 4096, uncounted and counted: 5.2 and 4.6 with 8 tokens, 5.7 and 5.6
+  // with 12, 7.6 and 7.9 with 32).
+  constexpr bool kCounted = NT <= 2;
+  // not a variable of its own, which would move all else off its 128-byte boundaries
+  uint64_t* const all_arrived = reinterpret_cast<uint64_t*>(smem + C::SMEM - 8);
+  if (threadIdx.x == 0) expect_sums(all_arrived, MATS * split * mine * 4);
+  cluster_arrive_relaxed();  // all CTAs of the cluster are ready for sums once this is waited for
 
   const char* src[MATS];  // the warp's next block
 #pragma unroll
@@ -382,7 +390,6 @@ w4_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, int acti
 
   copies_wait<0>();
   __syncthreads();  // the stages are done with
-  constexpr int kRows = kWarps * kTileRows, OUTPUTS = C::OUTPUTS;
   constexpr int kPitch = kRows + 4, kMatrix = 8 * NT * kPitch;  // four tokens of a warp's store hit different banks
   float* sums = reinterpret_cast<float*>(smem);                 // [matrix][token][row]
 #pragma unroll
@@ -395,27 +402,33 @@ w4_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, int acti
             acc[q][j][e] * (1.0f / H::kUnit);
   __syncthreads();
 
-  // Of the outputs [token][row] that exist each rank finishes `slice` (a multiple of 4).
-  const int outputs = (int)s.m * kRows, slice = s.slice;
   const float* arrived = reinterpret_cast<const float*>(smem + DEPTH * C::STAGE);
   const int begin = split > 1 ? rank * slice : 0;
+  bool in_time = true;
+  cluster_wait();
   if (split > 1) {
     const uint32_t arrivals = smem_addr + DEPTH * C::STAGE;  // [matrix][rank][slice]
-    cluster_wait();
 #pragma unroll 1
     for (int o = 4 * threadIdx.x; o < outputs; o += 128 * kWarps) {
       const int owner = (int)((unsigned)o / (unsigned)slice), at = rank * slice + o - owner * slice;
 #pragma unroll
-      for (int a = 0; a < MATS; ++a)
-        cluster_store4(arrivals + (a * (OUTPUTS + 64) + at) * 4, owner,
-                       *reinterpret_cast<const float4*>(sums + a * kMatrix + o / kRows * kPitch + o % kRows));
+      for (int a = 0; a < MATS; ++a) {
+        const uint32_t to = arrivals + (a * (OUTPUTS + 64) + at) * 4;
+        const float4& v = *reinterpret_cast<const float4*>(sums + a * kMatrix + o / kRows * kPitch + o % kRows);
+        if constexpr (kCounted) cluster_send4(to, tc::smem_u32(all_arrived), owner, v);
+        else cluster_store4(to, owner, v);
+      }
     }
-    cluster_arrive();
+    if constexpr (kCounted) {
+      in_time = mine <= 0 || own_wait(all_arrived, 0);
+    } else {
+      cluster_arrive();
+      cluster_wait();
+    }
   }
-  cluster_wait();
   const Consts consts(gm, dm);
 #pragma unroll 1
-  for (int o = 4 * threadIdx.x; o < slice && begin + o < outputs; o += 128 * kWarps) {
+  for (int o = 4 * threadIdx.x; o < mine; o += 128 * kWarps) {
     const int row = (begin + o) % kRows, tok = (begin + o) / kRows;
     const long long n = (long long)row_tile0 * kTileRows + row;
     if (n >= s.n) continue;
@@ -431,6 +444,7 @@ w4_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, int acti
       }
       v[0][a] = f.x, v[1][a] = f.y, v[2][a] = f.z, v[3][a] = f.w;
     }
+    if (!in_time) v[0][0] = v[1][0] = v[2][0] = v[3][0] = __uint_as_float(0x7fffffffu);
     store_results<T, MATS>(y, tok * s.y_pitch, n, s, v, activation, consts);
   }
 }
@@ -1319,8 +1333,8 @@ int run(void* y, const void* x, const W4* w, W4Shape s, int64_t m, int64_t x_row
         return launch_digits<T, MATS, G, 4>(y, x, w, s, activation, gm, dm, st);
       }
       // A launch of w4_mma_kernel starts and ends about 1 us slower, one of w4_kernel takes longer for each weight and 8 tokens
-      // (us, w4_kernel and w4_mma_kernel: 4096 -> 4096 with 8 tokens 5.2 and 6.2, with 32 7.6 and 8.4, with 64 12.1 and 11.9;
-      // 14336 -> 4096 with 8 tokens 11.6 and 11.4, with 16 13.9 and 11.8, with 32 19.3 and 13.3): lines through these times
+      // (us, w4_kernel and w4_mma_kernel: 4096 -> 4096 with 8 tokens 4.6 and 6.2, with 32 7.6 and 8.4, with 64 12.1 and 11.9;
+      // 14336 -> 4096 with 8 tokens 11.2 and 11.3, with 16 13.0 and 11.8, with 32 19.3 and 13.3): lines through these times
       // cross at this many weights.
       if (m > 32 || ((double)s.n * (double)s.k * MATS - 0x1p24) * (double)((m + 7) / 8 * 8) >= 0x1p28) {
         if (m <= 16) return launch_mma<T, MATS, 16, G>(y, x, w, s, activation, gm, dm, st);

@@ -256,7 +256,7 @@ def w4_linear(x: torch.Tensor, weight: W4Weight) -> torch.Tensor:
     m = x.numel() // k
     if m > LINEAR_ROWS:
         return x @ weight.dequantize().t()
-    y = x.new_empty((*x.shape[:-1], n))
+    y = x.new_empty((m, n) if x.dim() == 2 else (*x.shape[:-1], n))
     x, pitch = _aligned_rows(x)
     device = x.device
     _lib.check(
@@ -300,7 +300,7 @@ def w4_gate_up(x: torch.Tensor, w_gate: W4Weight, w_up: W4Weight, activation: st
     m = x.numel() // k
     if m > GATE_UP_ROWS:
         return _gate_up_16bit(x, w_gate, w_up, activation, gm, dm)
-    h = x.new_empty((*x.shape[:-1], n))
+    h = x.new_empty((m, n) if x.dim() == 2 else (*x.shape[:-1], n))
     x, pitch = _aligned_rows(x)
     device = x.device
     _lib.check(
