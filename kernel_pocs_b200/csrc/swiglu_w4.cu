@@ -64,6 +64,8 @@ template <> struct Half2<__nv_bfloat16> {
   // takes the zero point off; all of it is exact.
   static constexpr uint32_t kLow = 0x7f007f00u, kHigh = 0x7d007d00u;  // 2^127, 2^123
   static constexpr float kUnit = 0x1p-6f;
+  // Magnitudes above this one, as a float's bits, are whole multiples of 2^(e-156): 8 bits from 2^(e-149) on.
+  static __device__ __forceinline__ uint32_t whole_above(int e) { return ((uint32_t)(e - 22) << 23) - 1u; }
   static __device__ __forceinline__ uint32_t pair(float f) {
     __nv_bfloat162 v = __floats2bfloat162_rn(f, f);
     return *reinterpret_cast<uint32_t*>(&v);
@@ -82,6 +84,8 @@ template <> struct Half2<__half> {
   using V = __half2;
   static constexpr uint32_t kLow = 0x78007800u, kHigh = 0x68006800u;  // 2^15, 2^11; the step of the subnormals is 2^-24
   static constexpr float kUnit = 0x1p-9f;
+  // As above with 11 bits; up to e = 132 the unit is no more than 2^-24, of which every number is a multiple.
+  static __device__ __forceinline__ uint32_t whole_above(int e) { return e <= 132 ? 0u : ((uint32_t)(e - 19) << 23) - 1u; }
   static __device__ __forceinline__ uint32_t pair(float f) {
     __half2 v = __floats2half2_rn(f, f);
     return *reinterpret_cast<uint32_t*>(&v);
@@ -735,15 +739,24 @@ w4_mma_kernel(void* y, const __grid_constant__ Maps maps, W4 w0, W4 w1, W4Shape 
 // ------------------------------------------------------------------ one or two tokens: digits and integer products
 
 // As bytes the 8 nibbles of a word are two registers after three instructions (9 and four multiply-adds above), and
-// m16n8k32 multiplies them as they are.  For that a token is written as three 8-bit digits of a 23-bit number: with
-// 2^e above the largest magnitude of its 256 columns, X = rint(x * 2^(22-e)) = d0 + 2^8 d1 + 2^16 d2, the digits
-// balanced around zero.  Its digits are three columns of the product, so two tokens fill the eight columns of one
+// m16n8k32 multiplies them as they are.  For that a token is written as four 8-bit digits of a 31-bit number: with 2^e
+// above the largest magnitude of its 256 columns (a span), X = x * 2^(30-e) = d0 + 2^8 d1 + 2^16 d2 + 2^24 d3, the digits
+// balanced around zero.  Its digits are four columns of the product, so two tokens fill the eight columns of one
 // instruction.  Within a group the sums of nibble * digit are exact in 32 bits, the zero point comes off as z times the
-// digits' own sum (exact as well), and what is left, below 2^19, goes on in fp32: times the group's scale and 2^(8i+e-22).
-// A column is thus rounded by at most 2^-23 of the largest one beside it, which is what summing in fp32 does to it;
-// 16-bit numbers within 2^12 (fp16) or 2^15 (bf16) of the largest are exact.  A token with an Inf or a NaN gives NaN.
+// digits' own sum (exact as well), and what is left, below 2^19, goes on in fp32: times the group's scale and 2^(8i+e-30).
+//
+// X is a whole number, nothing of x is lost, for bf16 within 2^22 of the largest magnitude of the span and for fp16 within
+// 2^19, or wherever that magnitude is below 64.  It has to be: where the weight of a large column is zero, the small ones
+// beside it are the result.  A single token has the other four columns as well, for the digits of what X leaves over,
+// another 31 bits below.  With two tokens, or where 62 bits are too few (or the numbers below 2^-63, whose unit would leave
+// fp32), the span takes the 16-bit products of the kernels above, with the weights where they are: its unit is zero as a
+// mark, so its digits add nothing.
+//
+// us without such a span / with one / with one in every span: bf16 1 x 14336 -> 4096 7.9 / 8.2 / 8.7, gate and up
+// 1 x 4096 -> 14336 13.0 / 13.2 / 13.8, two tokens 4096 -> 11008 13.3 / 16.5 / 31.2.  Products silu(g) u of normal numbers
+// have one in 0.3 % of their spans in bf16 and in none in fp16.
 
-constexpr int kDigitTokens = 2, kDigitCols = 3 * kDigitTokens;
+constexpr int kDigitTokens = 2, kDigits = 4, kDigitCols = kDigits * kDigitTokens;
 constexpr int kSlab = 16;                              // column tiles whose digits are kept at a time, in pairs
 
 // A CTA: ROW_WARPS row tiles, whose pairs of column tiles are dealt to the warps that are left over.
@@ -769,23 +782,54 @@ __device__ __forceinline__ void imma(uint32_t (&d)[4], uint32_t a0, uint32_t a1,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Largest magnitude of eight 16-bit numbers as the bit pattern of a float.
-template <class T> __device__ __forceinline__ uint32_t top_of(const Vec<16>& v);
-template <> __device__ __forceinline__ uint32_t top_of<__nv_bfloat16>(const Vec<16>& v) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) m = max(m, max(v.w[i] << 16 & 0x7fffffffu, v.w[i] & 0x7fff0000u));
-  return m;
-}
-template <> __device__ __forceinline__ uint32_t top_of<__half>(const Vec<16>& v) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) m = max(m, max(v.w[i] & 0x7fffu, v.w[i] >> 16 & 0x7fffu));
-  return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
-}
-
 constexpr float kIntMagic = 12582912.0f;  // 1.5 * 2^23: added to an integer below 2^22, its bits are 0x4b400000 + it
 constexpr uint32_t kIntMagicBits = 0x4b400000u;
+
+// The 16-bit products of a span.  `block` is its first block of weights in shared memory, one of `tiles`; at `token` is the
+// place of its digits, where those of a marked token are the token itself, 16 bytes where the first two digits of its
+// eight columns would be.  Column g of B is token g; those whose bit 2 g is not in `marked` are zero.  The sums, of rows g and
+// g + 8 in units of kUnit, are returned to the lanes that hold the first digits: to t = 0 token 0's, to t = 2 token 1's.
+// A function of its own: as a part of the loop that rarely calls it, it took that 5 % of its time.
+template <class T, int GROUPS>
+__device__ __noinline__ float2 span_products(const unsigned char* block, bool zeros, const unsigned char* token, int tiles,
+                                             uint32_t marked) {
+  using H = Half2<T>;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const bool mine = g < kDigitTokens && marked >> (2 * g) & 1;
+  token += ((g & 1) * kDigits * 4 + t) * 16;
+  float sum[4] = {};
+#pragma unroll 1
+  for (int h = 0; h < tiles; ++h, block += block_bytes(GROUPS, zeros), token += 2 * kDigitCols * 64)
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {  // 32 columns each
+    const int at = (g * GROUPS + u * GROUPS / 4) * 2;
+    const unsigned char* tail = block + kTileBytes;
+    const uint4 b = mine ? *reinterpret_cast<const uint4*>(token + ((u >> 1) * kDigitCols + (u & 1)) * 64)
+                         : make_uint4(0u, 0u, 0u, 0u);
+    uint32_t bias_lo = H::pair(-8.0f * H::kUnit), bias_hi = bias_lo;
+    if (zeros) {
+      const uint32_t z = *reinterpret_cast<const uint16_t*>(tail + GROUPS * 32 + at);
+      bias_lo = H::pair(-H::kUnit * zero_point(z & 0xffu));
+      bias_hi = H::pair(-H::kUnit * zero_point(z >> 8));
+    }
+    uint32_t wl[4], wh[4];
+    weight_pairs<T>(*reinterpret_cast<const uint32_t*>(block + lane * 16 + 4 * u), bias_lo, wl);
+    weight_pairs<T>(*reinterpret_cast<const uint32_t*>(block + 512 + lane * 16 + 4 * u), bias_hi, wh);
+    const uint32_t a0[4] = {wl[0], wh[0], wl[1], wh[1]}, a1[4] = {wl[2], wh[2], wl[3], wh[3]};
+    float part[4];
+    H::mma(part, a0, b.x, b.y, 0.0f, 0.0f, 0.0f, 0.0f);
+    H::mma(part, a1, b.z, b.w, part[0], part[1], part[2], part[3]);
+    const uint32_t sc = *reinterpret_cast<const uint32_t*>(tail + at * 2);
+    const float s_lo = H::to_float(sc & 0xffffu), s_hi = H::to_float(sc >> 16);
+    sum[0] = fmaf(part[0], s_lo, sum[0]);
+    sum[1] = fmaf(part[1], s_lo, sum[1]);
+    sum[2] = fmaf(part[2], s_hi, sum[2]);
+    sum[3] = fmaf(part[3], s_hi, sum[3]);
+  }
+  // the lanes t = 0 have the sums of both tokens
+  const float lo = __shfl_sync(0xffffffffu, sum[1], lane & 28), hi = __shfl_sync(0xffffffffu, sum[3], lane & 28);
+  return t == 0 ? make_float2(sum[0], sum[2]) : t == 2 ? make_float2(lo, hi) : make_float2(0.0f, 0.0f);
+}
 
 // A CTA owns ROW_WARPS row tiles of MATS matrices, up to two tokens and, as rank r of a cluster of `split` CTAs, the
 // r-th part of the pairs of column tiles.  The code is kept short (loops that are not unrolled): a launch lasts a few
@@ -820,7 +864,7 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
   if (threadIdx.x == 0) expect_sums(sums, MATS * COL_WARPS * split * mine * 4);
   cluster_arrive_relaxed();  // all CTAs of the cluster are ready for sums once this is waited for
 
-  // This thread's eight columns of a token, of the slab that starts at pair p.
+  // This thread's eight columns of a token, of the slab that starts at pair p; zeros past the last one.
   auto read_token = [&](int p, int tok) {
     const long long k = (long long)p * (2 * kTileCols) + 8 * threadIdx.x;
     const char* src = cbyte(x) + (tok * s.x_pitch + k) * 2;
@@ -837,43 +881,68 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
     }
     return v;
   };
-  // Writes its digits, and what goes with them.
-  auto write_digits = [&](const Vec<16>& v, int tok) {
+  // Writes the digits of part `part` of a span, `f`: with two tokens a part is a token, with one it is the token and then what
+  // its digits left over.  A warp holds one span.  True when there is another part, which is then in `f` with one token.
+  auto write_digits = [&](const Vec<16>& token, float (&f)[8], int part) {
     const int piece = threadIdx.x & 15, tile = threadIdx.x >> 4, u = piece >> 2;
-    const int e = (int)(__reduce_max_sync(0xffffffffu, top_of<T>(v)) >> 23);  // the magnitudes are below 2^(e - 126)
-    if (lane < 3) units[warp * 8 + 3 * tok + lane] = e == 255 ? __uint_as_float(0x7fffffffu) : ldexpf(1.0f, e - 148 + 8 * lane);
-    const int up = 148 - e, half = up >> 1;  // 2^up as a product of two floats
-    const float f1 = __uint_as_float((uint32_t)(half + 127) << 23), f2 = __uint_as_float((uint32_t)(up - half + 127) << 23);
-    float f[8];
-    Codec<T>::template unpack<16>(v, f);
-    uint32_t z[8];  // bytes 0, 1, 2: the digits
+    uint32_t top = 0, below = 0xffffffffu;  // the largest magnitude, the least one but zero less one
 #pragma unroll
-    for (int a = 0; a < 8; ++a)
-      z[a] = (__float_as_uint(fmaf(f[a] * f1, f2, kIntMagic)) + (0x8080u - kIntMagicBits)) ^ 0x8080u;
-    int total[3];
-#pragma unroll
-    for (int d = 0; d < 3; ++d) {
-      // in the order of the nibbles: even ones columns 0, 4, 1, 5, odd ones 2, 6, 3, 7
-      const uint32_t pick = d | (4 + d) << 4;
-      const uint32_t even = __byte_perm(__byte_perm(z[0], z[4], pick), __byte_perm(z[1], z[5], pick), 0x5410);
-      const uint32_t odd = __byte_perm(__byte_perm(z[2], z[6], pick), __byte_perm(z[3], z[7], pick), 0x5410);
-      total[d] = __dp4a((int)even, 0x01010101, __dp4a((int)odd, 0x01010101, 0));
-      *reinterpret_cast<uint2*>(digits + (((tile * 2 + (u >> 1)) * kDigitCols + 3 * tok + d) * 4 + (piece & 3)) * 16 +
-                                (u & 1) * 8) = make_uint2(even, odd);
+    for (int a = 0; a < 8; ++a) {
+      const uint32_t magnitude = __float_as_uint(f[a]) & 0x7fffffffu;
+      top = max(top, magnitude);
+      below = min(below, magnitude - 1u);
     }
+    const int e = max((int)(__reduce_max_sync(0xffffffffu, top) >> 23), 64);  // the magnitudes are below 2^(e - 126)
+    const float up = __uint_as_float((uint32_t)(283 - e) << 23);  // 2^(156-e)
+    const bool whole = __all_sync(0xffffffffu, below >= H::whole_above(e));
+    uint32_t z[8];  // bytes: the digits
+#pragma unroll
+    for (int a = 0; a < 8; ++a) z[a] = ((uint32_t)__float2int_rn(f[a] * up) + 0x80808080u) ^ 0x80808080u;
+    const bool marked = !whole && part + 1 >= kDigitTokens / tokens && e != 255;
+    if (const int d = lane - kDigits * part; lane < kDigitCols && (d >= 0 || (marked && tokens == 1)))
+      units[warp * kDigitCols + lane] = e == 255                ? __uint_as_float(0x7fffffffu)
+                                        : marked || d >= kDigits ? 0.0f
+                                                                 : __uint_as_float((uint32_t)(e - 29 + 8 * d) << 23);
+    // digits of four columns to a word, in the order of the nibbles: even ones columns 0, 4, 1, 5, odd ones 2, 6, 3, 7
+    uint32_t digit[2][kDigits];
+#pragma unroll
+    for (int odd = 0; odd < 2; ++odd) {
+      const uint32_t a0 = __byte_perm(z[2 * odd], z[2 * odd + 4], 0x5140), a1 = __byte_perm(z[2 * odd], z[2 * odd + 4], 0x7362);
+      const uint32_t b0 = __byte_perm(z[2 * odd + 1], z[2 * odd + 5], 0x5140);
+      const uint32_t b1 = __byte_perm(z[2 * odd + 1], z[2 * odd + 5], 0x7362);
+      digit[odd][0] = __byte_perm(a0, b0, 0x5410);
+      digit[odd][1] = __byte_perm(a0, b0, 0x7632);
+      digit[odd][2] = __byte_perm(a1, b1, 0x5410);
+      digit[odd][3] = __byte_perm(a1, b1, 0x7632);
+    }
+    unsigned char* to = digits + ((tile * 2 + (u >> 1)) * kDigitCols * 4 + (piece & 3)) * 16;
+    int total[kDigits];
+#pragma unroll
+    for (int d = 0; d < kDigits; ++d) {
+      total[d] = __dp4a((int)digit[0][d], 0x01010101, __dp4a((int)digit[1][d], 0x01010101, 0));
+      if (!marked)
+        *reinterpret_cast<uint2*>(to + (kDigits * part + d) * 64 + (u & 1) * 8) = make_uint2(digit[0][d], digit[1][d]);
+    }
+    if (marked)
+      *reinterpret_cast<uint4*>(to + ((tokens == 1 ? 0 : kDigits * part) + (u & 1)) * 64) =
+          make_uint4(token.w[0], token.w[1], token.w[2], token.w[3]);
     // sums over the 4, 8 or 16 threads of a group; two of them travel in one register (each below 2^15)
-    int both = total[0] + (total[1] << 16);
+    int low = total[0] + (total[1] << 16), high = total[2] + (total[3] << 16);
 #pragma unroll
     for (int d = 1; d < 16 / GROUPS; d *= 2) {
-      both += __shfl_xor_sync(0xffffffffu, both, d);
-      total[2] += __shfl_xor_sync(0xffffffffu, total[2], d);
+      low += __shfl_xor_sync(0xffffffffu, low, d);
+      high += __shfl_xor_sync(0xffffffffu, high, d);
     }
-    if (piece % (16 / GROUPS) == 0) {
-      float* to = digit_sums + (threadIdx.x / (16 / GROUPS)) * 8 + 3 * tok;
-      to[0] = (float)(short)both;
-      to[1] = (float)((both - (short)both) >> 16);
-      to[2] = (float)total[2];
-    }
+    if (piece % (16 / GROUPS) == 0)
+      *reinterpret_cast<float4*>(digit_sums + (threadIdx.x / (16 / GROUPS)) * kDigitCols + kDigits * part) =
+          make_float4((float)(short)low, (float)((low - (short)low) >> 16), (float)(short)high,
+                      (float)((high - (short)high) >> 16));
+    if (part == 1 || tokens == 2) return part == 0;
+    if (whole || e == 255) return false;
+    const float down = __uint_as_float((uint32_t)(e - 29) << 23);
+#pragma unroll
+    for (int a = 0; a < 8; ++a) f[a] = fmaf(-(float)__float2int_rn(f[a] * up), down, f[a]);  // a difference of multiples of its last bit
+    return true;
   };
 
   // The warp's ring of pairs of blocks.
@@ -910,6 +979,9 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
     prefetch_l2(cbyte(mine.blocks) + ((long long)row_tile * s.col_tiles + 2 * first) * bytes,
                 min((DEPTH - 1) * COL_WARPS * 2, min(2 * last, s.col_tiles) - 2 * first) * bytes);
   }
+  // sums of the second part's digits where there is none: its unit is zero, and these have to be finite
+  if (tokens == 1 && threadIdx.x % (16 / GROUPS) == 0)
+    *reinterpret_cast<float4*>(digit_sums + (threadIdx.x / (16 / GROUPS)) * kDigitCols + kDigits) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   wait_for_previous();
   Vec<16> token = read_token(first, 0);
 #pragma unroll 1
@@ -923,12 +995,14 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
       __syncthreads();  // the digits have been read by all
       token = read_token(slab, 0);
     }
+    float f[8];
+    Codec<T>::template unpack<16>(token, f);
 #pragma unroll 1
-    for (int tok = 0;;) {
-      write_digits(token, tok);
-      if (++tok == tokens) break;
-      token = read_token(slab, tok);
-    }
+    for (int part = 0; write_digits(token, f, part); ++part)
+      if (tokens == 2) {
+        token = read_token(slab, 1);
+        Codec<T>::template unpack<16>(token, f);
+      }
     __syncthreads();
     const int end = last < slab + kSlab / 2 ? last : slab + kSlab / 2;
 #pragma unroll 1
@@ -942,8 +1016,7 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
       for (int h = 0; h < 2; ++h) {
         if (2 * p + h == s.col_tiles) break;
         const int in_slab = 2 * (p - slab) + h;
-        // lanes whose column is past the last digit read the first one's; nobody reads their sums
-        const unsigned char* piece = digits + (in_slab * 2 * kDigitCols * 4 + (g < kDigitCols ? lane : t)) * 16;
+        const unsigned char* piece = digits + (in_slab * 2 * kDigitCols * 4 + lane) * 16;
         const uint4 b0 = *reinterpret_cast<const uint4*>(piece);
         const uint4 b1 = *reinterpret_cast<const uint4*>(piece + kDigitCols * 64);
         const uint32_t b[4][2] = {{b0.x, b0.y}, {b0.z, b0.w}, {b1.x, b1.y}, {b1.z, b1.w}};
@@ -980,6 +1053,18 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
           }
         }
       }
+      // by the lanes t = 0 and t = 2, which hold the first digits of token 0 and of token 1
+      const uint32_t marked = __ballot_sync(0xffffffffu, unit.x == 0.0f) & (tokens == 1 ? 1u : 5u);
+      if (marked) {
+        const unsigned char* token = digits + (p - slab) * (4 * kDigitCols * 64);
+#pragma unroll
+        for (int a = 0; a < MATS; ++a) {
+          const float2 add = span_products<T, GROUPS>(ring + take + a * C::SLOT + (place[a] & 127u), w[a].zeros != 0, token,
+                                                      min(2, s.col_tiles - 2 * p), marked);
+          acc[a][0] = fmaf(add.x, 1.0f / H::kUnit, acc[a][0]);
+          acc[a][2] = fmaf(add.y, 1.0f / H::kUnit, acc[a][2]);
+        }
+      }
       take = take == (DEPTH - 1) * C::PAIR ? 0 : take + C::PAIR;
 #pragma unroll
       for (int a = 0; a < MATS; ++a) place[a] += 2 * COL_WARPS * block_bytes(GROUPS, w[a].zeros);
@@ -987,16 +1072,17 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
   }
 
   copies_wait<0>();
-  // A token's three columns, added up: token 0 is columns 0, 1, 2 and ends up in lanes t = 0, token 1 in lanes t = 1.
+  // A token's columns, added up: with two tokens one has the lanes t = 0 and 1 and the other t = 2 and 3, with one it has all.
   const uint32_t arrivals = smem_addr + C::RING + C::DIGITS + C::SUMS + C::UNITS;
   float* leaving = reinterpret_cast<float*>(smem + warp * (DEPTH * C::PAIR));  // [matrix][token][row] of this warp
 #pragma unroll
   for (int a = 0; a < MATS; ++a)
 #pragma unroll
     for (int hi = 0; hi < 2; ++hi) {
-      const float c0 = acc[a][2 * hi], c1 = acc[a][2 * hi + 1];
-      const float above = __shfl_down_sync(0xffffffffu, c0, 1), both = __shfl_down_sync(0xffffffffu, c0 + c1, 1);
-      if (t < tokens) leaving[(a * kDigitTokens + t) * kTileRows + g + 8 * hi] = t == 0 ? c0 + c1 + above : c1 + both;
+      const float own = acc[a][2 * hi] + acc[a][2 * hi + 1], four = own + __shfl_down_sync(0xffffffffu, own, 1);
+      const float eight = four + __shfl_down_sync(0xffffffffu, four, 2);
+      if (t % 2 == 0 && t / 2 < tokens)
+        leaving[(a * kDigitTokens + t / 2) * kTileRows + g + 8 * hi] = tokens == 1 ? eight : four;
     }
   __syncwarp();
   cluster_wait();
