@@ -355,8 +355,8 @@ SWIGLU_B200_API int swiglu_b200_ckpt8_bwd(void* h, void* dgate, void* dup, const
  *   y, h     m x n, row stride given; may not overlap x or the weights
  *   group    32, 64 or 128 columns share a scale
  * Meant for m up to a few hundred: every 64 tokens go through the weights again.  n and k are at most 2^30.  One or two
- * tokens are multiplied as integers wherever these hold every bit of their numbers (a token with an Inf or a NaN gives
- * NaN); the rest goes through 16-bit products with fp32 sums.  The order of every sum is fixed.  A wait inside a kernel that gives
+ * tokens are multiplied as integers wherever these hold every bit of their numbers; the rest goes through 16-bit products
+ * with fp32 sums.  The order of every sum is fixed.  A wait inside a kernel that gives
  * up, after half a second, turns the results of its CTA to NaN.
  * A call's kernel may start while the kernel of the linear / gate_up call before it on the stream is finishing; it reads
  * and writes nothing of the caller's until everything enqueued earlier is complete. */

@@ -749,7 +749,7 @@ w4_mma_kernel(void* y, const __grid_constant__ Maps maps, W4 w0, W4 w1, W4Shape 
 // 2^19, or wherever that magnitude is below 64.  It has to be: where the weight of a large column is zero, the small ones
 // beside it are the result.  A single token has the other four columns as well, for the digits of what X leaves over,
 // another 31 bits below.  With two tokens, or where 62 bits are too few (or the numbers below 2^-63, whose unit would leave
-// fp32), the span takes the 16-bit products of the kernels above, with the weights where they are: its unit is zero as a
+// fp32, or not finite), the span takes the 16-bit products of the kernels above, with the weights where they are: its unit is zero as a
 // mark, so its digits add nothing.
 //
 // us without such a span / with one / with one in every span: bf16 1 x 14336 -> 4096 7.9 / 8.2 / 8.7, gate and up
@@ -894,15 +894,13 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
     }
     const int e = max((int)(__reduce_max_sync(0xffffffffu, top) >> 23), 64);  // the magnitudes are below 2^(e - 126)
     const float up = __uint_as_float((uint32_t)(283 - e) << 23);  // 2^(156-e)
-    const bool whole = __all_sync(0xffffffffu, below >= H::whole_above(e));
+    const bool whole = __all_sync(0xffffffffu, below >= H::whole_above(e)) && e != 255;
     uint32_t z[8];  // bytes: the digits
 #pragma unroll
     for (int a = 0; a < 8; ++a) z[a] = ((uint32_t)__float2int_rn(f[a] * up) + 0x80808080u) ^ 0x80808080u;
-    const bool marked = !whole && part + 1 >= kDigitTokens / tokens && e != 255;
+    const bool marked = !whole && (part + 1 >= kDigitTokens / tokens || e == 255);
     if (const int d = lane - kDigits * part; lane < kDigitCols && (d >= 0 || (marked && tokens == 1)))
-      units[warp * kDigitCols + lane] = e == 255                ? __uint_as_float(0x7fffffffu)
-                                        : marked || d >= kDigits ? 0.0f
-                                                                 : __uint_as_float((uint32_t)(e - 29 + 8 * d) << 23);
+      units[warp * kDigitCols + lane] = marked || d >= kDigits ? 0.0f : __uint_as_float((uint32_t)(e - 29 + 8 * d) << 23);
     // digits of four columns to a word, in the order of the nibbles: even ones columns 0, 4, 1, 5, odd ones 2, 6, 3, 7
     uint32_t digit[2][kDigits];
 #pragma unroll
@@ -938,7 +936,7 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
           make_float4((float)(short)low, (float)((low - (short)low) >> 16), (float)(short)high,
                       (float)((high - (short)high) >> 16));
     if (part == 1 || tokens == 2) return part == 0;
-    if (whole || e == 255) return false;
+    if (whole || marked) return false;
     const float down = __uint_as_float((uint32_t)(e - 29) << 23);
 #pragma unroll
     for (int a = 0; a < 8; ++a) f[a] = fmaf(-(float)__float2int_rn(f[a] * up), down, f[a]);  // a difference of multiples of its last bit

@@ -94,3 +94,27 @@ def test_tokens_smaller_than_the_normal_range_of_their_unit(m):
     x = (tokens(m, k, torch.bfloat16).float() * 2.0 ** -100).to(torch.bfloat16)
     x[0, 256:] = 0.0
     assert_linear(w4_linear(x, w), x, w64, k, group)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m", [1, 2, 3, 12])
+@pytest.mark.parametrize("k,group,zeros", [(300, 64, True), (256, 128, False), (2100, 32, True)])
+def test_infinities_and_nan_go_through_the_formula(dtype, m, k, group, zeros):
+    """An Inf gives Inf of the weight's sign, and NaN where its weight is zero or another Inf is against it; a NaN gives NaN.
+    Every row has what the formula in float64 has, whatever the number of tokens."""
+    n = 90
+    w, w64 = blind_weight(n, k, group, zeros, dtype, (7,), seed=k)
+    clean = tokens(m, k, dtype)
+    at = min(k - 1, 1500)
+    for values in ({7: float("inf")}, {at: float("-inf")}, {7: float("inf"), at: float("inf")}, {at: float("nan")},
+                   {c: float("-inf") for c in range(8)}, {c: float("inf") for c in range(k)}):
+        x = clean.clone()
+        for c, v in values.items():
+            x[m - 1, c] = v
+        y = w4_linear(x, w).cpu().double()
+        want = (x.cpu().double()[:, None, :] * w64).sum(-1)
+        assert torch.equal(y.isnan(), want.isnan())
+        assert torch.equal(y.isinf() & (y > 0), want == float("inf"))
+        assert torch.equal(y.isinf() & (y < 0), want == float("-inf"))
+        assert torch.equal(y[:m - 1], w4_linear(clean, w).cpu().double()[:m - 1])
