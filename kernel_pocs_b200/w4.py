@@ -273,6 +273,8 @@ def _gate_up_16bit(x, w_gate, w_up, activation, gm, dm):
     from .geglu import gate_up_geglu_forward, geglu_forward
     from .swiglu import swiglu_forward
 
+    if x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)  # the fused projections start at 16-byte boundaries
     wg, wu = w_gate.dequantize(), w_up.dequantize()
     n, k = wg.shape
     approximate = "tanh" if activation == "gelu_tanh" else "none"
