@@ -11,12 +11,14 @@ numbers inside the kernel that multiplies them:
     W4Weight(packed, scales, zeros, ...) one from codes that exist already
 
 W[n, k] is ``(code - zero) * scale``; products with x are summed in fp32 and scaled in fp32, and the result is rounded
-once to the dtype of x.  Up to ``LINEAR_ROWS`` / ``GATE_UP_ROWS`` tokens take these kernels; more (a prompt) take the
-weights written out in 16 bits by ``W4Weight.dequantize`` and a library product, or the tensor-core projections of
-``fused_mlp`` / ``geglu``, whose operands then carry one more rounding (half a unit of the 16-bit type per weight).
-Forward only: weights are frozen and an input that wants a gradient is refused.  The reference has no counterpart (its inference path is bf16,
-kernels/lora_mlp/experiments/v5/lora_mlp_kernel_v5.py:451-454).  There is no path for tensors that are not on a CUDA
-device.
+once to the dtype of x, with any number of tokens.  Up to ``LINEAR_ROWS`` / ``GATE_UP_ROWS`` tokens take these kernels;
+more (a prompt) take the weights written out in 16 bits by ``W4Weight.dequantize``, one more rounding per weight (half a
+unit of the 16-bit type), and a library product or, for bf16 gate and up, the tensor-core projections of ``fused_mlp`` /
+``geglu``.  Those are not for a graph capture, nor for ``k % 8`` or ``n % 16``: the library takes their place there, with
+sums in another order, so that a captured prompt may differ from an eager one in the last bit.
+Forward only: weights are frozen and an input that wants a gradient is refused.  The reference has no counterpart (its
+inference path is bf16, kernels/lora_mlp/experiments/v5/lora_mlp_kernel_v5.py:451-454).  There is no path for tensors that
+are not on a CUDA device.
 """
 from __future__ import annotations
 
@@ -35,6 +37,10 @@ TILE_ROWS, TILE_COLS, CODE_BYTES = 16, 128, 1024
 # the weights again for every 64 tokens).  Linear 14336 -> 4096: 39.6 / 56.0 with 256 tokens, 70.5 / 65.9 with 384; 4096
 # -> 4096: 16.3 / 17.9 and 25.9 / 20.0.  Gate and up 4096 -> 14336: 149.3 / 154.5 with 448, 171.0 / 155.0 with 512.
 LINEAR_ROWS, GATE_UP_ROWS = 256, 448
+# Tokens of a prompt whose fp32 projections are held at a time where the library makes them.  In 16 bits the projections
+# would take less time (fp16 gate and up 4096 -> 11008: 116 instead of 131 us with 512 tokens, 325 instead of 367 with
+# 2048), but they would be rounded before the activation, and Inf above 65504.
+PIECE_ROWS = 4096
 
 
 def _ceil(a: int, b: int) -> int:
@@ -268,30 +274,34 @@ def w4_linear(x: torch.Tensor, weight: W4Weight) -> torch.Tensor:
 
 
 def _gate_up_16bit(x, w_gate, w_up, activation, gm, dm):
-    """The same stage from weights written out in 16 bits, for more tokens than the 4-bit kernels are for."""
+    """The same stage from weights written out in 16 bits, for more tokens than the 4-bit kernels are for.  Here too the
+    projections stay in fp32 up to the activation."""
     from .fused_mlp import gate_up_swiglu_forward
     from .geglu import gate_up_geglu_forward, geglu_forward
     from .swiglu import swiglu_forward
 
-    if x.data_ptr() % 16:
-        x = x.clone(memory_format=torch.contiguous_format)  # the fused projections start at 16-byte boundaries
     wg, wu = w_gate.dequantize(), w_up.dequantize()
     n, k = wg.shape
     approximate = "tanh" if activation == "gelu_tanh" else "none"
     # the fused projections report through status words that belong to launches, not to a graph's replays
     if x.dtype == torch.bfloat16 and k % 8 == 0 and n % 16 == 0 and not torch.cuda.is_current_stream_capturing():
+        if x.data_ptr() % 16:
+            x = x.clone(memory_format=torch.contiguous_format)  # they start at 16-byte boundaries
         if activation == "silu":
             return gate_up_swiglu_forward(x, wg, wu, gm, dm)
         return gate_up_geglu_forward(x, wg, wu, approximate)
-    gate, up = x @ wg.t(), x @ wu.t()
-    return swiglu_forward(gate, up, gm, dm)[0] if activation == "silu" else geglu_forward(gate, up, approximate)[0]
+    h = x.new_empty((*x.shape[:-1], n))
+    for rows, out in zip(x.reshape(-1, k).split(PIECE_ROWS), h.view(-1, n).split(PIECE_ROWS)):
+        gate, up = (torch.mm(rows, w.t(), out_dtype=torch.float32) for w in (wg, wu))
+        out.copy_(swiglu_forward(gate, up, gm, dm)[0] if activation == "silu" else geglu_forward(gate, up, approximate)[0])
+    return h
 
 
 def w4_gate_up(x: torch.Tensor, w_gate: W4Weight, w_up: W4Weight, activation: str = "silu",
                gate_multiplier: float = 1.0, down_multiplier: float = 1.0) -> torch.Tensor:
     """``act(x Wg^T * gate_multiplier) * (x Wu^T) * down_multiplier``; both projections and the activation (``"silu"``,
-    ``"gelu_tanh"`` or ``"gelu_exact"``; the GELU forms have no multipliers) in one launch, neither projection rounded
-    on the way."""
+    ``"gelu_tanh"`` or ``"gelu_exact"``; the GELU forms have no multipliers) in one launch up to ``GATE_UP_ROWS`` tokens;
+    the projections are not rounded to 16 bits on the way, however many there are."""
     _check_activation(activation)
     gm, dm = _check_multipliers(activation, gate_multiplier, down_multiplier)
     n, k = w_gate.out_features, w_gate.in_features
