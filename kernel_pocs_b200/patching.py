@@ -27,7 +27,10 @@ list).  It is opt-in: ``patch(model, kernels=["fused_gate_up", "swiglu"])`` or `
 Three more, opt-in as well, hold the block in fewer bits.  ``"swiglu_ckpt8"`` / ``"geglu_ckpt8"`` route the activation
 through ``checkpoint8``, which keeps gate and up in 8 bits for the backward, and ``"lora_mlp_fused_ckpt8"`` is
 ``"lora_mlp_fused"`` with the same; ``"mlp_w4"`` quantises the three projections (plain, bias-free, bf16 or fp16) to 4
-bits when the model is patched and runs the block from those: for generating, forward only.
+bits when the model is patched and runs the block from those: for generating, forward only (with gradients enabled it
+refuses an input or projections that want one).  The 4-bit weights are kept beside the module's own, which ``unpatch``
+needs: they follow the input to another device, are in no ``state_dict``, and see no later change of the weights; hooks of
+the projections are not called.
 """
 from __future__ import annotations
 
@@ -247,6 +250,10 @@ def make_mlp_w4_forward(module) -> Callable:
     weights = [quantize_w4(proj.weight) for proj in projections]
 
     def forward(x):
+        # an x that wants a gradient is refused further down; these would be left without theirs
+        if torch.is_grad_enabled() and any(proj.weight.requires_grad for proj in projections):
+            raise RuntimeError("mlp_w4 is forward only (frozen 4-bit weights): call the model under torch.no_grad(), or "
+                               "with requires_grad off for its projections")
         if weights[0].device != x.device:
             weights[:] = [w.to(x.device) for w in weights]
         return w4_mlp(x, *weights, activation)
