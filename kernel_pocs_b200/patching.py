@@ -294,7 +294,8 @@ def patch(model, kernels: Optional[List[str]] = None):
         if name not in FORWARD_MAKERS:
             raise KeyError(f"patch: unknown kernel {name!r}. Known: {sorted(FORWARD_MAKERS)}.")
 
-    originals: dict = {}
+    # all forwards are made before any is bound: one that cannot be made leaves the model as it was
+    made: list = []
     counts: Dict[str, int] = {}
     for _name, module in model.named_modules():
         if type(module).__name__ not in mlp_classes:
@@ -304,11 +305,14 @@ def patch(model, kernels: Optional[List[str]] = None):
                 new_forward = FORWARD_MAKERS[name](module)
             except SkipPatch:
                 continue
-            originals[id(module)] = (module, module.forward)
-            module.forward = new_forward
+            made.append((module, new_forward))
             counts[name] = counts.get(name, 0) + 1
             break
 
+    originals: dict = {}
+    for module, new_forward in made:
+        originals[id(module)] = (module, module.forward)
+        module.forward = new_forward
     model._forge_originals = originals
     model._forge_patched = True
     model._forge_patched_counts = counts

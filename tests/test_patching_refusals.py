@@ -41,3 +41,20 @@ def test_frozen_4_bit_projections_run_with_gradients_enabled():
         p.requires_grad_()
     with pytest.raises(RuntimeError, match="forward only"):
         model(ids)
+
+
+@pytest.mark.parametrize("make", [tiny_qwen3, tiny_gemma2])
+def test_a_patch_that_fails_leaves_the_model_as_it_was(make):
+    """The second layer cannot be quantised: nothing of the first one stays behind, and the model can be patched anew."""
+    model = make(torch.bfloat16)
+    mlp = model.model.layers[1].mlp
+    with torch.no_grad():
+        kept = mlp.down_proj.weight[3, 5].clone()
+        mlp.down_proj.weight[3, 5] = float("nan")
+    with pytest.raises(ValueError, match="not finite"):
+        patching.patch(model, kernels=["mlp_w4"])
+    assert all("forward" not in vars(layer.mlp) for layer in model.model.layers)
+    assert not hasattr(model, "_forge_originals") and not getattr(model, "_forge_patched", False)
+    with torch.no_grad():
+        mlp.down_proj.weight[3, 5] = kept
+    assert patching.patch(model, kernels=["mlp_w4"])._forge_patched_counts == {"mlp_w4": 2}
