@@ -216,13 +216,15 @@ def quantize_w4(weight: torch.Tensor, group_size: int = 128, zero_points: bool =
             scale = (w.abs().amax(-1) / 7).to(dtype)
         if not bool(torch.isfinite(scale).all()):
             raise ValueError(f"weight holds magnitudes whose scale is not a finite {dtype}")
-        inverse = torch.where(scale > 0, 1.0 / scale.to(torch.float32), 0.0)
+        # 1 / scale leaves fp32 for scales below 2^-128: these are lifted, with their weights, by a power of two
+        lift = torch.where(scale < 2.0 ** -100, 2.0 ** 60, 1.0).to(torch.float32)
+        inverse = torch.where(scale > 0, 1.0 / (scale.to(torch.float32) * lift), 0.0)
         if zero_points:
-            zero = torch.round(-low * inverse).clamp(0, 15)
+            zero = torch.round(-(low * lift) * inverse).clamp(0, 15)
             zeros[lo:lo + step] = zero.to(torch.uint8)
         else:
             zero = torch.full_like(inverse, 8.0)
-        code = (torch.round(w * inverse.unsqueeze(-1)) + zero.unsqueeze(-1)).clamp(0, 15).to(torch.uint8)
+        code = (torch.round(w * lift.unsqueeze(-1) * inverse.unsqueeze(-1)) + zero.unsqueeze(-1)).clamp(0, 15).to(torch.uint8)
         code = torch.nn.functional.pad(code.view(rows, -1), (0, max(0, pitch - groups * group_size)))[:, :pitch]
         packed[lo:lo + step] = code[:, 0::2] | (code[:, 1::2] << 4)
         scales[lo:lo + step] = scale
