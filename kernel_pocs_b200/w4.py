@@ -161,8 +161,10 @@ class W4Weight:
         return self._blocks.numel()
 
     def to(self, device) -> "W4Weight":
-        """This weight on ``device`` (itself when it is there already)."""
-        moved = self._blocks.to(device)
+        """This weight on ``device`` (itself when it is there already).  Its type cannot be changed."""
+        if not isinstance(device, (str, int, torch.device)):
+            raise TypeError(f"W4Weight.to takes a device, got {device!r}")
+        moved = self._blocks.to(torch.device(device))
         if moved is self._blocks:
             return self
         other = object.__new__(W4Weight)

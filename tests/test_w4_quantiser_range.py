@@ -1,8 +1,8 @@
-"""quantize_w4 at the ends of the types' ranges."""
+"""quantize_w4 at the ends of the types' ranges, and W4Weight.to."""
 import pytest
 import torch
 
-from kernel_pocs_b200.w4 import quantize_w4
+from kernel_pocs_b200.w4 import W4Weight, quantize_w4
 from tests.test_w4 import random_parts, weight64
 
 
@@ -42,3 +42,13 @@ def test_the_device_gives_the_codes_of_the_host(dtype, size, zero_points):
     # a product may be rounded to the other side of half a step by the last bit of an inverse, no further
     off = (weight64(device.packed, device.scales, device.zeros, 300, 64) - weight64(host.packed, host.scales, host.zeros, 300, 64)).abs()
     assert bool((off <= host.scales.double()[:, torch.arange(300) // 64]).all()) and float((off > 0).double().mean()) < 0.01
+
+
+def test_to_moves_and_does_not_convert():
+    w = W4Weight(*random_parts(20, 70, 32, True, torch.bfloat16), in_features=70, group_size=32)
+    assert w.to("cpu") is w and w.to(torch.device("cpu")) is w and w.to(device="cpu") is w
+    meta = w.to("meta")
+    assert meta.device.type == "meta" and meta.blocks.dtype == torch.uint8 and meta.shape == w.shape
+    for other in (torch.float16, torch.uint8, torch.zeros(1, dtype=torch.float16), None):
+        with pytest.raises(TypeError, match="device"):
+            w.to(other)
