@@ -329,7 +329,7 @@ SWIGLU_B200_API int swiglu_b200_ckpt8_fwd(void* h, void* gate_codes, void* up_co
  *                  block that needs h again (a LoRA MLP); may overwrite dout exactly (same address, same stride)
  *   dgate, dup     rows x cols, row stride grad_row_stride (dup = dgate + cols in the packed layout)
  *   dout           rows x cols, row stride dout_row_stride
- * No other overlap between an output and an input or h is allowed. */
+ * No other overlap between an output and an input or another output is allowed. */
 SWIGLU_B200_API int swiglu_b200_ckpt8_bwd(void* h, void* dgate, void* dup, const void* dout, const void* gate_codes,
                           const void* up_codes, const void* gate_steps, const void* up_steps, int64_t rows,
                           int64_t cols, int64_t grad_row_stride, int64_t dout_row_stride, int64_t h_row_stride,

@@ -43,6 +43,17 @@ inline ByteRange byte_range(const void* p, long long rows, long long row_bytes, 
   return ByteRange{address(p), address(p) + (unsigned long long)((rows - 1) * pitch_bytes + row_bytes)};
 }
 inline bool overlap(const ByteRange& a, const ByteRange& b) { return a.lo < b.hi && b.lo < a.hi; }
+// Whether two sets of rows at one pitch share a byte.  Their rows may lie between one another's, as the two halves of a
+// packed tensor do.
+inline bool rows_overlap(const void* p, const void* q, long long rows, long long row_bytes, long long pitch_bytes) {
+  const unsigned long long a = address(p), b = address(q);
+  const unsigned long long apart = a < b ? b - a : a - b;
+  if (rows <= 1) return apart < (unsigned long long)row_bytes;
+  const unsigned long long skipped = apart / (unsigned long long)pitch_bytes;  // rows before the one it falls into
+  const unsigned long long into = apart % (unsigned long long)pitch_bytes;
+  return (skipped < (unsigned long long)rows && into < (unsigned long long)row_bytes) ||
+         (skipped + 1 < (unsigned long long)rows && into + (unsigned long long)row_bytes > (unsigned long long)pitch_bytes);
+}
 
 // True when rows * pitch (in bytes) and everything derived from it stays within 62 bits.
 inline bool fits_address_space(long long rows, long long pitch, long long element) {

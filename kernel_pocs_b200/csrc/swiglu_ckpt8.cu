@@ -483,10 +483,10 @@ int swiglu_b200_ckpt8_bwd(void* h, void* dgate, void* dup, const void* dout, con
     const ByteRange in[4] = {byte_range(gate_codes, 1, rows * groups * kGroup, 0),
                              byte_range(up_codes, 1, rows * groups * kGroup, 0),
                              byte_range(gate_steps, 1, rows * groups, 0), byte_range(up_steps, 1, rows * groups, 0)};
-    // interleaved rows of a packed dgate|dup buffer overlap each other as ranges, rightly
+    // rows of a packed dgate|dup buffer lie between one another's: as ranges the two overlap rightly
     const ByteRange grad[2] = {byte_range(dgate, rows, cols * es, grad_row_stride * es),
                                byte_range(dup, rows, cols * es, grad_row_stride * es)};
-    if (dgate == dup) return SWIGLU_B200_ERR_ALIAS;
+    if (rows_overlap(dgate, dup, rows, cols * es, grad_row_stride * es)) return SWIGLU_B200_ERR_ALIAS;
     const ByteRange hr = h ? byte_range(h, rows, cols * es, h_row_stride * es) : ByteRange{0, 0};
     const bool over_dout = h == dout && h_row_stride == dout_row_stride;
     for (const ByteRange& g : grad)
