@@ -5,12 +5,21 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "swiglu_b200.h"
+
 namespace swiglu_b200 {
 
 // Counts one kernel launch in swiglu_b200_launch_count().
 void note_launch();
 // Records `e` for swiglu_b200_last_cuda_error() and returns `code`.
 int note_cuda_error(int code, cudaError_t e);
+// The code of a launch that was just made, which is counted.
+inline int launched() {
+  const cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess) return note_cuda_error(SWIGLU_B200_ERR_LAUNCH, err);
+  note_launch();
+  return SWIGLU_B200_OK;
+}
 
 // Makes `device` current for the duration of a call (no-op for -1 or when it already is).
 struct CallDevice {

@@ -76,25 +76,6 @@ int fail_cuda(int code, cudaError_t e) {
   return code;
 }
 
-struct DeviceScope {
-  // Makes `device` current for the duration of a call (no-op for -1 or when it already is).
-  int prev = -1;
-  bool switched = false;
-  cudaError_t err = cudaSuccess;
-  explicit DeviceScope(int device) {
-    if (device < 0) return;
-    err = cudaGetDevice(&prev);
-    if (err != cudaSuccess) return;
-    if (prev != device) {
-      err = cudaSetDevice(device);
-      switched = (err == cudaSuccess);
-    }
-  }
-  ~DeviceScope() {
-    if (switched) cudaSetDevice(prev);
-  }
-};
-
 constexpr long long kMaxGrid = 0x7fffffffLL;  // gridDim.x limit
 
 unsigned grid_for(long long n_vec, int threads, int unroll) {
@@ -387,19 +368,8 @@ inline int plan_code(const Plan& p) {
          (p.ragged ? 1 << 11 : 0) | (p.shape.head << 16) | (p.shape.edge << 24);
 }
 
-inline unsigned long long addr_of(const void* p) { return (unsigned long long)(uintptr_t)p; }
 inline const void* advance(const void* p, long long bytes) { return static_cast<const char*>(p) + bytes; }
 inline void* advance(void* p, long long bytes) { return static_cast<char*>(p) + bytes; }
-
-// Byte extent [lo, hi) touched by a rows x cols tensor with the given row stride.
-struct Extent {
-  unsigned long long lo, hi;
-};
-inline Extent extent(const void* p, long long rows, long long cols, long long stride, int es) {
-  const unsigned long long lo = addr_of(p);
-  return Extent{lo, lo + (unsigned long long)(((rows - 1) * stride + cols) * es)};
-}
-inline bool overlaps(const Extent& a, const Extent& b) { return a.lo < b.hi && b.lo < a.hi; }
 
 }  // namespace
 
@@ -446,19 +416,19 @@ int fwd_entry(void* out, const void* gate, const void* up, int64_t rows, int64_t
   if (in_row_stride < cols || out_row_stride < cols) return SWIGLU_B200_ERR_SHAPE;
   if (!out || !gate || !up) return SWIGLU_B200_ERR_NULL;
   const int es = elem_size(dtype);
-  if (addr_of(out) % es || addr_of(gate) % es || addr_of(up) % es) return SWIGLU_B200_ERR_ALIGN;
+  if (address(out) % es || address(gate) % es || address(up) % es) return SWIGLU_B200_ERR_ALIGN;
   {
-    const Extent eo = extent(out, rows, cols, out_row_stride, es);
-    if (overlaps(eo, extent(gate, rows, cols, in_row_stride, es)) ||
-        overlaps(eo, extent(up, rows, cols, in_row_stride, es)))
+    const ByteRange eo = byte_range(out, rows, cols * es, out_row_stride * es);
+    if (overlap(eo, byte_range(gate, rows, cols * es, in_row_stride * es)) ||
+        overlap(eo, byte_range(up, rows, cols * es, in_row_stride * es)))
       return SWIGLU_B200_ERR_ALIAS;
   }
 
-  DeviceScope scope(device);
+  CallDevice scope(device);
   if (scope.err != cudaSuccess) return fail_cuda(SWIGLU_B200_ERR_DEVICE, scope.err);
 
-  const unsigned long long outs[1] = {addr_of(out)};
-  const unsigned long long ins[2] = {addr_of(gate), addr_of(up)};
+  const unsigned long long outs[1] = {address(out)};
+  const unsigned long long ins[2] = {address(gate), address(up)};
   const long long pitch[2] = {in_row_stride, out_row_stride};
   Plan p = make_plan(outs, 1, ins, 2, pitch, 2, rows, cols, es);
   p.shape.skew_gate = p.skew[0];
@@ -491,7 +461,7 @@ int bwd_entry(void* dgate, void* dup, const void* dout, const void* gate, const 
   if (in_row_stride < cols || grad_row_stride < cols || dout_row_stride < cols) return SWIGLU_B200_ERR_SHAPE;
   if (!dgate || !dup || !dout || !gate || !up) return SWIGLU_B200_ERR_NULL;
   const int es = elem_size(dtype);
-  if (addr_of(dgate) % es || addr_of(dup) % es || addr_of(dout) % es || addr_of(gate) % es || addr_of(up) % es)
+  if (address(dgate) % es || address(dup) % es || address(dout) % es || address(gate) % es || address(up) % es)
     return SWIGLU_B200_ERR_ALIGN;
 
   // Either both gradients overwrite their inputs exactly, or no output touches any input.
@@ -502,25 +472,25 @@ int bwd_entry(void* dgate, void* dup, const void* dout, const void* gate, const 
     inplace = true;
   }
   {
-    const Extent edg = extent(dgate, rows, cols, grad_row_stride, es);
-    const Extent edu = extent(dup, rows, cols, grad_row_stride, es);
-    const Extent ed = extent(dout, rows, cols, dout_row_stride, es);
-    if (overlaps(edg, ed) || overlaps(edu, ed)) return SWIGLU_B200_ERR_ALIAS;
+    const ByteRange edg = byte_range(dgate, rows, cols * es, grad_row_stride * es);
+    const ByteRange edu = byte_range(dup, rows, cols * es, grad_row_stride * es);
+    const ByteRange ed = byte_range(dout, rows, cols * es, dout_row_stride * es);
+    if (overlap(edg, ed) || overlap(edu, ed)) return SWIGLU_B200_ERR_ALIAS;
     if (!inplace) {
-      const Extent eg = extent(gate, rows, cols, in_row_stride, es);
-      const Extent eu = extent(up, rows, cols, in_row_stride, es);
+      const ByteRange eg = byte_range(gate, rows, cols * es, in_row_stride * es);
+      const ByteRange eu = byte_range(up, rows, cols * es, in_row_stride * es);
       // Interleaved rows of a packed buffer make the bounding extents of dgate and dup
       // overlap each other legitimately; only input/output overlap is an error.
-      if (overlaps(edg, eg) || overlaps(edg, eu) || overlaps(edu, eg) || overlaps(edu, eu))
+      if (overlap(edg, eg) || overlap(edg, eu) || overlap(edu, eg) || overlap(edu, eu))
         return SWIGLU_B200_ERR_ALIAS;
     }
   }
 
-  DeviceScope scope(device);
+  CallDevice scope(device);
   if (scope.err != cudaSuccess) return fail_cuda(SWIGLU_B200_ERR_DEVICE, scope.err);
 
-  const unsigned long long outs[2] = {addr_of(dgate), addr_of(dup)};
-  const unsigned long long ins[3] = {addr_of(dout), addr_of(gate), addr_of(up)};  // in place: gate/up == outs
+  const unsigned long long outs[2] = {address(dgate), address(dup)};
+  const unsigned long long ins[3] = {address(dout), address(gate), address(up)};  // in place: gate/up == outs
   const long long pitch[3] = {in_row_stride, grad_row_stride, dout_row_stride};
   Plan p = make_plan(outs, 2, ins, 3, pitch, 3, rows, cols, es);
   p.shape.skew_dout = p.skew[0];
@@ -558,22 +528,22 @@ int recompute_entry(void* h, void* dgate, void* dup, const void* dout, const voi
   const void* ins[3] = {dout, gate, up};
   int width = 16;
   for (int k = 0; k < 3; ++k) {
-    if (addr_of(outs[k]) % es || addr_of(ins[k]) % es) return SWIGLU_B200_ERR_ALIGN;
-    width = pow2_divisor(addr_of(outs[k]), width);
-    width = pow2_divisor(addr_of(ins[k]), width);
+    if (address(outs[k]) % es || address(ins[k]) % es) return SWIGLU_B200_ERR_ALIGN;
+    width = pow2_divisor(address(outs[k]), width);
+    width = pow2_divisor(address(ins[k]), width);
   }
   // An output may overwrite one input exactly; any other overlap (outputs with each other included) is an error.
   bool aliased = false;
   for (int a = 0; a < 3; ++a) {
-    const Extent ea = extent(outs[a], 1, n, n, es);
+    const ByteRange ea = byte_range(outs[a], 1, n * es, 0);
     for (int b = a + 1; b < 3; ++b)
-      if (overlaps(ea, extent(outs[b], 1, n, n, es))) return SWIGLU_B200_ERR_ALIAS;
+      if (overlap(ea, byte_range(outs[b], 1, n * es, 0))) return SWIGLU_B200_ERR_ALIAS;
     for (int b = 0; b < 3; ++b) {
       if (outs[a] == ins[b]) aliased = true;
-      else if (overlaps(ea, extent(ins[b], 1, n, n, es))) return SWIGLU_B200_ERR_ALIAS;
+      else if (overlap(ea, byte_range(ins[b], 1, n * es, 0))) return SWIGLU_B200_ERR_ALIAS;
     }
   }
-  DeviceScope scope(device);
+  CallDevice scope(device);
   if (scope.err != cudaSuccess) return fail_cuda(SWIGLU_B200_ERR_DEVICE, scope.err);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (dtype) {
@@ -643,9 +613,9 @@ int swiglu_b200_plan_fwd(const void* out, const void* gate, const void* up, int6
   if (dtype != SWIGLU_B200_F32 && dtype != SWIGLU_B200_F16 && dtype != SWIGLU_B200_BF16) return -SWIGLU_B200_ERR_DTYPE;
   if (rows <= 0 || cols <= 0 || in_row_stride < cols || out_row_stride < cols) return -SWIGLU_B200_ERR_SHAPE;
   const int es = elem_size(dtype);
-  if (addr_of(out) % es || addr_of(gate) % es || addr_of(up) % es) return -SWIGLU_B200_ERR_ALIGN;
-  const unsigned long long outs[1] = {addr_of(out)};
-  const unsigned long long ins[2] = {addr_of(gate), addr_of(up)};
+  if (address(out) % es || address(gate) % es || address(up) % es) return -SWIGLU_B200_ERR_ALIGN;
+  const unsigned long long outs[1] = {address(out)};
+  const unsigned long long ins[2] = {address(gate), address(up)};
   const long long pitch[2] = {in_row_stride, out_row_stride};
   const Plan p = make_plan(outs, 1, ins, 2, pitch, 2, rows, cols, es);
   return plan_code(p);
@@ -658,10 +628,10 @@ int swiglu_b200_plan_bwd(const void* dgate, const void* dup, const void* dout, c
   if (rows <= 0 || cols <= 0 || in_row_stride < cols || grad_row_stride < cols || dout_row_stride < cols)
     return -SWIGLU_B200_ERR_SHAPE;
   const int es = elem_size(dtype);
-  if (addr_of(dgate) % es || addr_of(dup) % es || addr_of(dout) % es || addr_of(gate) % es || addr_of(up) % es)
+  if (address(dgate) % es || address(dup) % es || address(dout) % es || address(gate) % es || address(up) % es)
     return -SWIGLU_B200_ERR_ALIGN;
-  const unsigned long long outs[2] = {addr_of(dgate), addr_of(dup)};
-  const unsigned long long ins[3] = {addr_of(dout), addr_of(gate), addr_of(up)};
+  const unsigned long long outs[2] = {address(dgate), address(dup)};
+  const unsigned long long ins[3] = {address(dout), address(gate), address(up)};
   const long long pitch[3] = {in_row_stride, grad_row_stride, dout_row_stride};
   const Plan p = make_plan(outs, 2, ins, 3, pitch, 3, rows, cols, es);
   return plan_code(p);

@@ -37,7 +37,6 @@ constexpr uint32_t kNonFinite = 255;
 struct Ckpt8Shape {
   long long rows, cols;
   long long groups;      // per row; a row of codes takes 32 * groups bytes, a row of step exponents `groups`
-  int tasks_per_row;     // warp tasks of 32 frames
   long long pitch_in;    // bytes between rows of gate / up (forward) or dh (backward)
   long long pitch_out;   // bytes between rows of h
   long long pitch_grad;  // bytes between rows of dgate / dup
@@ -348,10 +347,9 @@ struct Grid {
 };
 
 // A CTA takes up to kWarps consecutive tasks of one row, the row's tasks spread evenly over its CTAs.
-Grid grid_of(Ckpt8Shape& s, int epv) {
+Grid grid_of(const Ckpt8Shape& s, int epv) {
   const long long frames = s.groups * (kGroup / epv);
   const long long tasks = (frames + 31) / 32;
-  s.tasks_per_row = (int)tasks;
   const long long ctas = (tasks + kWarps - 1) / kWarps;
   const long long warps = (tasks + ctas - 1) / ctas;
   const long long z = (s.rows + 65534) / 65535;
@@ -362,13 +360,6 @@ Grid grid_of(Ckpt8Shape& s, int epv) {
 
 bool known_dtype(int dtype) {
   return dtype == SWIGLU_B200_F32 || dtype == SWIGLU_B200_F16 || dtype == SWIGLU_B200_BF16;
-}
-
-int launched() {
-  const cudaError_t err = cudaGetLastError();
-  if (err != cudaSuccess) return note_cuda_error(SWIGLU_B200_ERR_LAUNCH, err);
-  note_launch();
-  return SWIGLU_B200_OK;
 }
 
 template <class F>

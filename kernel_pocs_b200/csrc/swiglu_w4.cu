@@ -1193,13 +1193,6 @@ __global__ void __launch_bounds__(32 * kOutTiles) w4_dequantize_rows_kernel(void
 
 // ------------------------------------------------------------------ host side
 
-int launched() {
-  const cudaError_t err = cudaGetLastError();
-  if (err != cudaSuccess) return note_cuda_error(SWIGLU_B200_ERR_LAUNCH, err);
-  note_launch();
-  return SWIGLU_B200_OK;
-}
-
 constexpr long long kMaxSize = 1LL << 30;  // of n and k: tile counts and copies' coordinates fit an int, byte offsets 62 bits
 
 // Checks shared by the three entries; fills the shape.
