@@ -265,7 +265,8 @@ def w4_linear(x: torch.Tensor, weight: W4Weight) -> torch.Tensor:
     n, k = weight.out_features, weight.in_features
     m = x.numel() // k
     if m > LINEAR_ROWS:
-        return x @ weight.dequantize().t()
+        with torch.autocast("cuda", enabled=False):  # which does not reach the 4-bit kernels either
+            return x @ weight.dequantize().t()
     y = x.new_empty((m, n) if x.dim() == 2 else (*x.shape[:-1], n))
     x, pitch = _aligned_rows(x)
     device = x.device
@@ -295,9 +296,11 @@ def _gate_up_16bit(x, w_gate, w_up, activation, gm, dm):
             return gate_up_swiglu_forward(x, wg, wu, gm, dm)
         return gate_up_geglu_forward(x, wg, wu, approximate)
     h = x.new_empty((*x.shape[:-1], n))
-    for rows, out in zip(x.reshape(-1, k).split(PIECE_ROWS), h.view(-1, n).split(PIECE_ROWS)):
-        gate, up = (torch.mm(rows, w.t(), out_dtype=torch.float32) for w in (wg, wu))
-        out.copy_(swiglu_forward(gate, up, gm, dm)[0] if activation == "silu" else geglu_forward(gate, up, approximate)[0])
+    with torch.autocast("cuda", enabled=False):
+        for rows, out in zip(x.reshape(-1, k).split(PIECE_ROWS), h.view(-1, n).split(PIECE_ROWS)):
+            gate, up = (torch.mm(rows, w.t(), out_dtype=torch.float32) for w in (wg, wu))
+            out.copy_((swiglu_forward(gate, up, gm, dm) if activation == "silu" else
+                       geglu_forward(gate, up, approximate))[0])
     return h
 
 

@@ -104,3 +104,17 @@ def test_a_prompt_is_worked_on_in_pieces(monkeypatch):
     monkeypatch.setattr(w4, "PIECE_ROWS", 128)
     # pieces may take other products of the library: sums in another order, rounded once
     torch.testing.assert_close(w4_gate_up(x, wg, wu), whole, rtol=2 * torch.finfo(dtype).eps, atol=1e-4)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,other", [(torch.float16, torch.bfloat16), (torch.bfloat16, torch.float16)])
+@pytest.mark.parametrize("m,n,k", [(8, 64, 256), (M, 64, 256), (M, 37, 129)])
+def test_autocast_does_not_reach_the_products(dtype, other, m, n, k):
+    wg, wu = make(n, k, 64, True, dtype)[0], make(n, k, 64, False, dtype, seed=9)[0]
+    x = tokens(m, k, dtype)
+    with torch.no_grad():
+        want = [w4_linear(x, wg), *(w4_gate_up(x, wg, wu, act, gm, dm) for act, gm, dm in ACTS)]
+        with torch.autocast("cuda", dtype=other):
+            got = [w4_linear(x, wg), *(w4_gate_up(x, wg, wu, act, gm, dm) for act, gm, dm in ACTS)]
+    check_status()
+    assert all(a.dtype == dtype and torch.equal(a, b) for a, b in zip(got, want))
