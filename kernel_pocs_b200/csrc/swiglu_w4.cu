@@ -462,7 +462,7 @@ w4_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, int acti
 // accesses to shared memory for a block), and the work for a weight is the same for any number of tokens.  The products
 // of a scale group are read back, and scaled and added up in registers.
 //
-// A kernel that allocates tensor memory runs with one CTA to an SM, so a CTA has four such warpgroups, which work on
+// A CTA takes an SM to itself (all 512 columns of tensor memory, 224 KB of stages) and has four such warpgroups, which work on
 // column tiles of their own.  While one waits for its products the others turn codes into numbers; what bounds the kernel
 // are the instructions for that (bf16 32 x 4096 -> 14336 gate and up: 84 % of the issue slots of the busy SMs).
 
