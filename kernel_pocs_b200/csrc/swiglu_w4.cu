@@ -921,9 +921,11 @@ w4_digits_kernel(void* y, const void* __restrict__ x, W4 w0, W4 w1, W4Shape s, i
       if (!marked)
         *reinterpret_cast<uint2*>(to + (kDigits * part + d) * 64 + (u & 1) * 8) = make_uint2(digit[0][d], digit[1][d]);
     }
-    if (marked)
+    if (marked) {
+      __syncwarp();  // over the first part's digits, other lanes' among them
       *reinterpret_cast<uint4*>(to + ((tokens == 1 ? 0 : kDigits * part) + (u & 1)) * 64) =
           make_uint4(token.w[0], token.w[1], token.w[2], token.w[3]);
+    }
     // sums over the 4, 8 or 16 threads of a group; two of them travel in one register (each below 2^15)
     int low = total[0] + (total[1] << 16), high = total[2] + (total[3] << 16);
 #pragma unroll
