@@ -1404,8 +1404,10 @@ int run(void* y, const void* x, const W4* w, W4Shape s, int64_t m, int64_t x_row
       constexpr int G = decltype(groups)::value;
       if (m <= kDigitTokens) {
         // 128 rows to a CTA leave it a shorter part of the tokens to make digits of, and can be split more evenly; 64 rows
-        // make more CTAs where there are few rows, and smaller clusters (us, 64 and 128: 1 x 5504 -> 11009 11.6 and 8.2,
-        // 14336 -> 4096 8.7 and 7.6, 4096 -> 4096 3.9 and 3.9, gate and up 2048 -> 4096 3.9 and 4.4, 8192 -> 2048 4.0 and 5.1).
+        // make more CTAs where there are few rows, and smaller clusters (us, 64 and 128: 5000 -> 6000 6.9 and 5.5, 6144 -> 4096
+        // 4.9 and 4.8, 2048 -> 4096 3.0 and 3.2, 8192 -> 2048 4.1 and 5.3, gate and up 4096 -> 11008 13.2 and 10.7, 2048 -> 5504
+        // 4.5 and 5.0).  Of 18 shapes between 1024 -> 2048 and 4096 -> 11008 the other side was faster by more than 2 % in two,
+        // gate and up 4096 -> 4096 (5.2 against 5.7) and 2048 -> 2048 (3.7 against 4.0).
         const long long pairs = (s.col_tiles + 1) / 2;
         if (pairs >= 16 && (s.n + 127) / 128 * 8 >= kEnoughCtas)
           return launch_digits<T, MATS, G, 8>(y, x, w, s, activation, gm, dm, st);
@@ -1414,7 +1416,9 @@ int run(void* y, const void* x, const W4* w, W4Shape s, int64_t m, int64_t x_row
       // A launch of w4_mma_kernel starts and ends about 1 us slower, one of w4_kernel takes longer for each weight and 8 tokens
       // (us, w4_kernel and w4_mma_kernel: 4096 -> 4096 with 8 tokens 4.6 and 6.2, with 32 7.6 and 8.4, with 64 12.1 and 11.9;
       // 14336 -> 4096 with 8 tokens 11.2 and 11.3, with 16 13.0 and 11.8, with 32 19.3 and 13.3): lines through these times
-      // cross at this many weights.
+      // cross at this many weights.  Of 48 cases in fp16 from 4 to 32 tokens and 2048 -> 4096 to 4096 -> 11008 the other side was
+      // faster by more than 4 % in five: 20 tokens 4096 -> 6144 (9.1 against 10.2) and gate and up of 2048 and 2731 square with
+      // 20 and 32 (5 to 9 %).
       if (m > 32 || ((double)s.n * (double)s.k * MATS - 0x1p24) * (double)((m + 7) / 8 * 8) >= 0x1p28) {
         if (m <= 16) return launch_mma<T, MATS, 16, G>(y, x, w, s, activation, gm, dm, st);
         if (m <= 32) return launch_mma<T, MATS, 32, G>(y, x, w, s, activation, gm, dm, st);
