@@ -118,3 +118,26 @@ def test_infinities_and_nan_go_through_the_formula(dtype, m, k, group, zeros):
         assert torch.equal(y.isinf() & (y > 0), want == float("inf"))
         assert torch.equal(y.isinf() & (y < 0), want == float("-inf"))
         assert torch.equal(y[:m - 1], w4_linear(clean, w).cpu().double()[:m - 1])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k,group,zeros", [(33, 130, 1000, 64, True), (64, 40, 520, 128, False), (100, 257, 264, 32, True)])
+def test_many_tokens_beside_large_channels_infinities_and_nan(dtype, m, n, k, group, zeros):
+    """The same of the tensor-core form: rows that do not see the large channels, and the formula for what is not finite."""
+    columns = (0, 77, k - 1)
+    w, w64 = blind_weight(n, k, group, zeros, dtype, columns, seed=k)
+    x = tokens(m, k, dtype).float() * 0.01
+    x[:, list(columns)] = 30000.0
+    x = x.to(dtype)
+    clean = w4_linear(x, w)
+    assert_linear(clean, x, w64, k, group)
+    x[1, 77], x[m - 1, 78], x[m // 2, 79] = float("inf"), float("-inf"), float("nan")
+    y = w4_linear(x, w)
+    hit = [1, m - 1, m // 2]
+    want = (x[hit].cpu().double()[:, None, :] * w64).sum(-1)
+    got = y[hit].cpu().double()
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.isinf() & (got > 0), want == float("inf")) and torch.equal(got.isinf() & (got < 0), want == -float("inf"))
+    keep = [i for i in range(m) if i not in hit]
+    assert torch.equal(y[keep], clean[keep])
